@@ -29,7 +29,9 @@ extern "C" {
 typedef void* pdae_stream_t; /* hipStream_t */
 
 const char* pdae_last_error(void);
-/* ABI history.  11 (round 6): + pdae_conv2d_wgrad_form (which kernel a weight gradient runs on); knobs PDAE_W3V, PDAE_Y_XCD, PDAE_Y_GRID_TRIM.
+/* ABI history.  11, extended without a new number (entry points and op kinds were only added; arrays and callers written for 11 run unchanged): + the token
+ *   operators pdae_layernorm_*, pdae_dropout_*, pdae_mha_* and their records PDAE_OP_LAYERNORM_FWD .. PDAE_OP_MHA_BWD.
+ * 11 (round 6): + pdae_conv2d_wgrad_form (which kernel a weight gradient runs on); knobs PDAE_W3V, PDAE_Y_XCD, PDAE_Y_GRID_TRIM.
  * 10 (round 5): pdae_op.reserved became pdae_op.flags (PDAE_OPF_SIDE: the executor's second stream) + PDAE_OP_JOIN + knob
  *   PDAE_SIDE_STREAM; arrays written for ABI 9 (flags = 0) run unchanged.
  * 9 (round 5): - pdae_wino_* (the gated 2-D Winograd probe left the library: tools/probes/r04_winograd/); + pdae_set_knob / pdae_get_knob
@@ -307,6 +309,52 @@ int pdae_attn_fwd(const float* qkv, int N, int T, int C, int heads, int new_orde
 int pdae_attn_bwd(const float* qkv, const float* out, const float* lse, const float* d_out, int N, int T, int C, int heads, int new_order, float* dqkv,
                   void* ws, pdae_stream_t stream);
 
+/* ---- token operators: layer norm, dropout and attention for any number of rows / tokens (layernorm.hip, dropout.hip, mha_fwd.hip, mha_bwd.hip).
+ * dtype: element type of the activations and their gradients, PDAE_F32 or PDAE_BF16; parameters, their gradients, statistics and every sum are fp32.
+ * Tensors need the alignment of their element only.  Nothing is allocated, cleared with a memset or synchronised: the calls can be captured into a graph.
+ * A workspace belongs to one call at a time: two calls (or captured graphs) that may run at once need one each. */
+#define PDAE_F32 0
+#define PDAE_BF16 1
+
+/* y = (x - mu) rstd gamma + beta per row of C channels (biased variance, rstd = 1 / sqrt(var + eps)); next to pdae_mlp_modln_* (which fuses the
+ * condition scale and SiLU of MLPSkipNet, fp32 only) this is the bare norm.  ldx / ldy: row strides in elements (>= C).  gamma, beta, mean, rstd may be NULL. */
+int pdae_layernorm_fwd(const void* x, int64_t ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, int64_t ldy, float* mean, float* rstd,
+                       int dtype, pdae_stream_t stream);
+/* dx = LayerNorm backward (+ add, the identity path around the norm); dgamma / dbeta (+)= sums over the rows, in a fixed order (acc_param selects "+=";
+ * either may be NULL; with both NULL no workspace is needed).  dx may be add; no other output may overlap an input. */
+size_t pdae_layernorm_workspace_bytes(int R, int C);
+int pdae_layernorm_bwd(const void* x, int64_t ldx, const float* gamma, const float* mean, const float* rstd, const void* dy, int64_t lddy, const void* add,
+                       int64_t ldadd, int R, int C, void* dx, int64_t lddx, float* dgamma, float* dbeta, int acc_param, void* ws, size_t ws_bytes, int dtype,
+                       pdae_stream_t stream);
+
+/* y = res + x * keep / (1 - p) over n contiguous elements (res may be NULL; y may be x or res) and dx (+)= dy * keep / (1 - p) (dx may be dy).
+ * keep is a pure function of (seed, offset, element index): Philox2x32 with ten rounds, counter = element >> 2, 16 bits per element, dropped when below
+ * round(p * 65536) -- the generator of pdae_gn_apply, and the same mask for the same (p, seed, offset).  Both directions compute it; no mask is
+ * stored.  offset: low 32 bits = step, high 32 bits = a number per call site (layer): masks of different layers of one step are different streams.
+ * In a pdae_op record step and layer are two integers.  0 <= p < 1.  A dropped element is an exact zero, whatever x holds. */
+int pdae_dropout_fwd(const void* x, const void* res, int64_t n, float p, uint64_t seed, uint64_t offset, void* y, int dtype, pdae_stream_t stream);
+int pdae_dropout_bwd(const void* dy, int64_t n, float p, uint64_t seed, uint64_t offset, void* dx, int accumulate, int dtype, pdae_stream_t stream);
+
+/* o[b][i][h] = sum_j p_ij v[b][j][h'],  p_i = softmax_j(scale q[b][i][h] . k[b][j][h']) over the keys row i sees,  h' = h / (Hq / Hkv).
+ * Key j is seen by query i of sample b iff j < k_len[b] and, when causal, j <= i + k_len[b] - q_len[b] (the last query sees every key).  q_len / k_len: device
+ * int32 [B] or NULL (all Tq / Tk); values outside [0, Tq] / [0, Tk] are cut.  A row that sees no key and a row behind q_len: o = 0, lse = -inf, gradients 0;
+ * rows of dk / dv behind k_len are 0.  Keys and queries behind the lengths are never read.  Keys that only `causal` hides are read (with finite values
+ * their weight is an exact 0; a non-finite value there may reach rows of the same 128-row tile).
+ * Strides in elements; channels are contiguous.  Gradients have their tensor's strides (d_o those of o, dq of q, dk of k, dv of v).
+ * Limits: D <= 128, Hq a multiple of Hkv, scale > 0.  Sums, softmax statistics and partial results fp32; bf16 tensors multiply in bf16 (probabilities and
+ * their gradients rounded to bf16 for the second product), fp32 tensors in three exact bf16 planes x six products.  Results are the same bits every run.
+ * lse [B][Hq][Tq] (natural log) may be NULL in the forward; the backward needs it and o.  ws: pdae_mha_workspace_bytes(d, backward). */
+typedef struct pdae_mha_desc {
+  int32_t B, Tq, Tk, Hq, Hkv, D, dtype, causal;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];   /* batch, token, head */
+  float scale;
+} pdae_mha_desc;
+size_t pdae_mha_workspace_bytes(const pdae_mha_desc* d, int backward);
+int pdae_mha_fwd(const pdae_mha_desc* d, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len, void* o, float* lse, void* ws,
+                 size_t ws_bytes, pdae_stream_t stream);
+int pdae_mha_bwd(const pdae_mha_desc* d, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len, const void* o, const float* lse,
+                 const void* d_o, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, pdae_stream_t stream);
+
 /* ---- evaluator (sampler/autoencoding_eval.py:83-99): per-image SSIM and MSE of two (N,C,H,W)-shaped batches of ANY strides in one pass.
  * Both inputs are mapped v -> v*mul + add first (the (x+1)/2 of autoencoding_eval.py:83-88: mul = add = 0.5).  SSIM = metric/utils.py:35-57
  * (11-tap Gaussian window, given normalised as window11 so that the caller controls its rounding; zero padding; C1 = 1e-4, C2 = 9e-4; mean over
@@ -355,7 +403,10 @@ enum {
   PDAE_OP_AXPBY_ROWS, PDAE_OP_DDIM_STEP_ROWS, PDAE_OP_DDPM_STEP_ROWS, PDAE_OP_LINEAR_GROUP,
   PDAE_OP_ATTN_FWD, PDAE_OP_ATTN_BWD, PDAE_OP_LINEAR_BWD_GROUP, PDAE_OP_GN_COEF_FROM_CONV_STATS, PDAE_OP_CONV_WPREP_GROUP,
   PDAE_OP_SUBSAMPLE2, PDAE_OP_ZERO_INSERT2, PDAE_OP_GN_STATS_QUADS,
-  PDAE_OP_JOIN     /* (ABI 10) the caller's stream waits for every PDAE_OPF_SIDE op issued so far; no arguments */
+  PDAE_OP_JOIN,    /* (ABI 10) the caller's stream waits for every PDAE_OPF_SIDE op issued so far; no arguments */
+  /* token operators.  i: LAYERNORM_FWD R, C, dtype, ldx, ldy;  LAYERNORM_BWD R, C, dtype, ldx, lddy, ldadd, lddx, acc_param, ws_bytes;  DROPOUT_FWD n, dtype,
+   * seed, step, layer;  DROPOUT_BWD + accumulate;  MHA_* the eight int32 of the descriptor, its twelve strides, ws_bytes (f[0] = scale) */
+  PDAE_OP_LAYERNORM_FWD, PDAE_OP_LAYERNORM_BWD, PDAE_OP_DROPOUT_FWD, PDAE_OP_DROPOUT_BWD, PDAE_OP_MHA_FWD, PDAE_OP_MHA_BWD
 };
 /* pdae_op.flags (ABI 10; the field was `reserved`, always 0).  PDAE_OPF_SIDE: issue this op on the executor's second (low-priority) stream.
  * It starts when the ops in front of it in the array have finished, and runs beside the ops behind it until the next PDAE_OP_JOIN or the end

@@ -9,6 +9,7 @@
 #include "igemm.h"
 #include "kernels.h"
 #include "conv3x3p.h"
+#include "mha.h"
 
 static thread_local char g_err[512] = "";
 
@@ -771,6 +772,102 @@ static void desc_from(const int64_t* i, pdae_conv_desc& d) {
   d.KH = (int)i[8]; d.KW = (int)i[9]; d.stride = (int)i[10]; d.pad = (int)i[11]; d.up = (int)i[12]; d.math = (int)i[13];
 }
 
+// ---- token operators
+extern "C" size_t pdae_layernorm_workspace_bytes(int R, int C) { return k_layernorm_workspace_bytes(R, C); }
+extern "C" int pdae_layernorm_fwd(const void* x, int64_t ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, int64_t ldy, float* mean,
+                                  float* rstd, int dtype, pdae_stream_t stream) {
+  return k_layernorm_fwd(x, ldx, gamma, beta, R, C, eps, y, ldy, mean, rstd, dtype, S(stream));
+}
+extern "C" int pdae_layernorm_bwd(const void* x, int64_t ldx, const float* gamma, const float* mean, const float* rstd, const void* dy, int64_t lddy, const void* add,
+                                  int64_t ldadd, int R, int C, void* dx, int64_t lddx, float* dgamma, float* dbeta, int acc_param, void* ws, size_t ws_bytes,
+                                  int dtype, pdae_stream_t stream) {
+  return k_layernorm_bwd(x, ldx, gamma, mean, rstd, dy, lddy, add, ldadd, R, C, dx, lddx, dgamma, dbeta, acc_param, ws, ws_bytes, dtype, S(stream));
+}
+extern "C" int pdae_dropout_fwd(const void* x, const void* res, int64_t n, float p, uint64_t seed, uint64_t offset, void* y, int dtype, pdae_stream_t stream) {
+  return k_dropout(x, res, n, p, seed, offset, y, dtype, S(stream));
+}
+extern "C" int pdae_dropout_bwd(const void* dy, int64_t n, float p, uint64_t seed, uint64_t offset, void* dx, int accumulate, int dtype, pdae_stream_t stream) {
+  return k_dropout(dy, accumulate ? dx : nullptr, n, p, seed, offset, dx, dtype, S(stream));
+}
+// no two (batch, token, head) rows of D channels share memory
+static bool mha_rows_disjoint(const int64_t* st, int n0, int n1, int n2, int D) {
+  long long s[3] = {st[0], st[1], st[2]}, n[3] = {n0, n1, n2};
+  if (n0 == 0 || n1 == 0 || n2 == 0) return true;
+  long long extent = D;
+  for (int pass = 0; pass < 3; ++pass) {
+    int k = -1;
+    for (int j = 0; j < 3; ++j)
+      if (n[j] > 1 && (k < 0 || s[j] < s[k])) k = j;
+    if (k < 0) break;
+    if (s[k] < extent) return false;
+    extent += s[k] * (n[k] - 1);
+    n[k] = 1;
+  }
+  return true;
+}
+static int mha_params(const pdae_mha_desc* d, int backward, MhaParams& P) {
+  PDAE_CHECK_ARG(d, "mha: null descriptor");
+  PDAE_CHECK_ARG(tk_dtype_ok(d->dtype), "mha: dtype must be 0 (fp32) or 1 (bf16), got %d", d->dtype);
+  PDAE_CHECK_ARG(d->B >= 0 && d->Tq >= 0 && d->Tk >= 0 && d->Hq > 0 && d->Hkv > 0, "mha: bad sizes (B %d, Tq %d, Tk %d, Hq %d, Hkv %d)", d->B, d->Tq, d->Tk, d->Hq, d->Hkv);
+  PDAE_CHECK_ARG(d->Hq % d->Hkv == 0, "mha: %d query heads cannot share %d key heads", d->Hq, d->Hkv);
+  PDAE_CHECK_ARG(d->D >= 1 && d->D <= 128, "mha: head width %d is not supported (1 .. 128)", d->D);
+  PDAE_CHECK_ARG(d->scale > 0.f && d->scale < 3.0e38f, "mha: scale must be positive and finite, got %g", (double)d->scale);
+  PDAE_CHECK_ARG((long long)d->B * d->Hq < (1ll << 30) && d->Tq < (1 << 30) && d->Tk < (1 << 30), "mha: too many heads or tokens");
+  for (int j = 0; j < 3; ++j)
+    for (const int64_t* st : {d->q_stride, d->k_stride, d->v_stride, d->o_stride})
+      PDAE_CHECK_ARG(st[j] >= 0 && st[j] < (1ll << 40), "mha: stride %lld is out of range", (long long)st[j]);
+  PDAE_CHECK_ARG(mha_rows_disjoint(d->o_stride, d->B, d->Tq, d->Hq, d->D), "mha: rows of o overlap (strides %lld, %lld, %lld)", (long long)d->o_stride[0],
+                 (long long)d->o_stride[1], (long long)d->o_stride[2]);
+  if (backward) {
+    PDAE_CHECK_ARG(mha_rows_disjoint(d->q_stride, d->B, d->Tq, d->Hq, d->D), "mha: rows of dq (the strides of q) overlap");
+    PDAE_CHECK_ARG(mha_rows_disjoint(d->k_stride, d->B, d->Tk, d->Hkv, d->D), "mha: rows of dk (the strides of k) overlap");
+    PDAE_CHECK_ARG(mha_rows_disjoint(d->v_stride, d->B, d->Tk, d->Hkv, d->D), "mha: rows of dv (the strides of v) overlap");
+  }
+  memset(&P, 0, sizeof(P));
+  P.B = d->B; P.Tq = d->Tq; P.Tk = d->Tk; P.Hq = d->Hq; P.Hkv = d->Hkv; P.G = d->Hq / d->Hkv; P.D = d->D; P.causal = d->causal != 0;
+  P.scale = d->scale; P.sc2 = d->scale * MH_LOG2E;
+  P.qb = d->q_stride[0]; P.qt = d->q_stride[1]; P.qh = d->q_stride[2]; P.kb = d->k_stride[0]; P.kt = d->k_stride[1]; P.kh = d->k_stride[2];
+  P.vb = d->v_stride[0]; P.vt = d->v_stride[1]; P.vh = d->v_stride[2]; P.ob = d->o_stride[0]; P.ot = d->o_stride[1]; P.oh = d->o_stride[2];
+  return PDAE_OK;
+}
+extern "C" size_t pdae_mha_workspace_bytes(const pdae_mha_desc* d, int backward) {
+  MhaParams P;
+  if (mha_params(d, 0, P)) return 0;
+  const size_t f = k_mha_fwd_workspace_bytes(P, d->dtype);
+  if (!backward) return f;
+  const size_t b = k_mha_bwd_workspace_bytes(P);
+  return b > f ? b : f;                          // one buffer serves the forward and the backward that follows it
+}
+extern "C" int pdae_mha_fwd(const pdae_mha_desc* d, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len, void* o, float* lse, void* ws,
+                            size_t ws_bytes, pdae_stream_t stream) {
+  MhaParams P;
+  if (int e = mha_params(d, 0, P)) return e;
+  const bool rows = P.B > 0 && P.Tq > 0, keys = P.B > 0 && P.Tk > 0;
+  PDAE_CHECK_ARG((!rows || (q && o)) && (!rows || !keys || (k && v)), "mha_fwd: null pointer");
+  PDAE_CHECK_ARG(tk_aligned(q, d->dtype) && tk_aligned(k, d->dtype) && tk_aligned(v, d->dtype) && tk_aligned(o, d->dtype) && tk_aligned(ws, PDAE_DT_F32),
+                 "mha_fwd: tensors must be aligned to their element size");
+  P.q = q; P.k = k; P.v = v; P.out = o; P.lse = lse; P.q_len = q_len; P.k_len = k_len;
+  return k_mha_fwd(P, d->dtype, ws, ws_bytes, S(stream));
+}
+extern "C" int pdae_mha_bwd(const pdae_mha_desc* d, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len, const void* o, const float* lse,
+                            const void* d_o, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes, pdae_stream_t stream) {
+  MhaParams P;
+  if (int e = mha_params(d, 1, P)) return e;
+  const bool rows = P.B > 0 && P.Tq > 0, keys = P.B > 0 && P.Tk > 0;
+  PDAE_CHECK_ARG((!rows || (q && o && lse && d_o && dq)) && (!keys || (k && v && dk && dv)), "mha_bwd: null pointer");
+  PDAE_CHECK_ARG(tk_aligned(q, d->dtype) && tk_aligned(k, d->dtype) && tk_aligned(v, d->dtype) && tk_aligned(o, d->dtype) && tk_aligned(d_o, d->dtype) &&
+                     tk_aligned(dq, d->dtype) && tk_aligned(dk, d->dtype) && tk_aligned(dv, d->dtype) && tk_aligned(ws, PDAE_DT_F32),
+                 "mha_bwd: tensors must be aligned to their element size");
+  P.q = q; P.k = k; P.v = v; P.o = o; P.lse = const_cast<float*>(lse); P.d_o = d_o; P.dq = dq; P.dk = dk; P.dv = dv; P.q_len = q_len; P.k_len = k_len;
+  return k_mha_bwd(P, d->dtype, ws, ws_bytes, S(stream));
+}
+static void mha_desc_from(const pdae_op& o, pdae_mha_desc& d) {
+  const int64_t* i = o.i;
+  d.B = (int)i[0]; d.Tq = (int)i[1]; d.Tk = (int)i[2]; d.Hq = (int)i[3]; d.Hkv = (int)i[4]; d.D = (int)i[5]; d.dtype = (int)i[6]; d.causal = (int)i[7];
+  for (int j = 0; j < 3; ++j) { d.q_stride[j] = i[8 + j]; d.k_stride[j] = i[11 + j]; d.v_stride[j] = i[14 + j]; d.o_stride[j] = i[17 + j]; }
+  d.scale = (float)o.f[0];
+}
+
 static int run_one(const pdae_op& o, pdae_stream_t st) {
   void* const* p = o.p; const int64_t* i = o.i; const double* f = o.f;
 #define F(k) ((const float*)p[k])
@@ -867,6 +964,25 @@ static int run_one(const pdae_op& o, pdae_stream_t st) {
       hipError_t e = hipMemcpyAsync(p[1], p[0], (size_t)i[0], hipMemcpyDeviceToDevice, S(st));
       if (e != hipSuccess) { pdae_set_error("copy: %s", hipGetErrorString(e)); return (int)e; }
       return PDAE_OK;
+    }
+    case PDAE_OP_LAYERNORM_FWD:
+      return pdae_layernorm_fwd(p[0], i[3], F(1), F(2), (int)i[0], (int)i[1], (float)f[0], p[3], i[4], FM(4), FM(5), (int)i[2], st);
+    case PDAE_OP_LAYERNORM_BWD:
+      return pdae_layernorm_bwd(p[0], i[3], F(1), F(2), F(3), p[4], i[4], p[5], i[5], (int)i[0], (int)i[1], p[6], i[6], FM(7), FM(8), (int)i[7], p[9], (size_t)i[8],
+                                (int)i[2], st);
+    case PDAE_OP_DROPOUT_FWD:
+      return pdae_dropout_fwd(p[0], p[1], i[0], (float)f[0], (uint64_t)i[2], (uint64_t)(uint32_t)i[3] | (uint64_t)i[4] << 32, p[2], (int)i[1], st);
+    case PDAE_OP_DROPOUT_BWD:
+      return pdae_dropout_bwd(p[0], i[0], (float)f[0], (uint64_t)i[2], (uint64_t)(uint32_t)i[3] | (uint64_t)i[4] << 32, p[1], (int)i[5], (int)i[1], st);
+    case PDAE_OP_MHA_FWD: {
+      pdae_mha_desc md;
+      mha_desc_from(o, md);
+      return pdae_mha_fwd(&md, p[0], p[1], p[2], (const int32_t*)p[5], (const int32_t*)p[6], p[3], FM(4), p[7], (size_t)i[20], st);
+    }
+    case PDAE_OP_MHA_BWD: {
+      pdae_mha_desc md;
+      mha_desc_from(o, md);
+      return pdae_mha_bwd(&md, p[0], p[1], p[2], (const int32_t*)p[9], (const int32_t*)p[10], p[3], F(4), p[5], p[6], p[7], p[8], p[11], (size_t)i[20], st);
     }
     default: pdae_set_error("run_ops: unknown op kind %d", o.kind); return PDAE_EINVAL;
   }

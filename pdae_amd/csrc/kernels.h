@@ -69,6 +69,20 @@ int k_attn_fwd(const float* qkv, int N, int T, int C, int heads, int new_order, 
 int k_attn_bwd(const float* qkv, const float* o, const float* lse, const float* d_o, int N, int T, int C, int heads, int new_order, float* dqkv,
                float* dvec, hipStream_t st);
 
+// dropout.hip / layernorm.hip / mha_fwd.hip / mha_bwd.hip (token operators)
+int k_dropout(const void* x, const void* add, long long n, float p, unsigned long long seed, unsigned long long offset, void* y, int dtype, hipStream_t st);
+size_t k_layernorm_workspace_bytes(int R, int C);
+int k_layernorm_fwd(const void* x, long long ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, long long ldy, float* mean, float* rstd,
+                    int dtype, hipStream_t st);
+int k_layernorm_bwd(const void* x, long long ldx, const float* gamma, const float* mean, const float* rstd, const void* dy, long long lddy, const void* add,
+                    long long ldadd, int R, int C, void* dx, long long lddx, float* dgamma, float* dbeta, int acc_param, void* ws, size_t ws_bytes, int dtype,
+                    hipStream_t st);
+struct MhaParams;
+size_t k_mha_fwd_workspace_bytes(const MhaParams& P, int dtype);
+size_t k_mha_bwd_workspace_bytes(const MhaParams& P);
+int k_mha_fwd(const MhaParams& P, int dtype, void* ws, size_t ws_bytes, hipStream_t st);
+int k_mha_bwd(const MhaParams& P, int dtype, void* ws, size_t ws_bytes, hipStream_t st);
+
 // comm.hip
 int k_comm_unique_id(const char* librccl_path, void* id128);
 int k_comm_init(const char* librccl_path, const void* id128, int nranks, int rank, void** comm);

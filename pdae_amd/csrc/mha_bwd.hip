@@ -1,0 +1,384 @@
+// Attention backward (mha.h): the probabilities are recomputed from q, k and the saved row log-sum-exp, nothing of size tokens x tokens exists.
+//
+//   delta[q] = sum_d dO[q][d] O[q][d]                         mha_delta_kernel
+//   P = exp(scale q.k - lse),  dP = dO.v,  dS = P (dP - delta)
+//   dV = P^T dO,  dK = scale dS^T Q                           mha_dkv_kernel: a wave owns 32 keys (columns), the queries stream through LDS
+//   dQ = scale dS K                                           mha_dq_kernel:  a wave owns 32 queries (columns), the keys stream through LDS
+//
+// Two kernels recompute S and dP twice (7 products of 2 Tq Tk D instead of 5): dK / dV and dQ then each have ONE writer, so there are no atomics and the
+// results are the same bits every run.  dK / dV of a key head sum over the query heads that share it inside the kernel.
+// Few tiles: the summed axis is split into ranges (grid `splits`), every range leaves an fp32 partial, mha_bwd_join_kernel adds them in order.
+// Row validity is decided where rows are staged: queries that do not exist or (causal) see no key come as zeros with lse = +inf, so P = 0 exactly and
+// non-finite values in them reach nothing.
+#include "kernels.h"
+#include "mha.h"
+
+// 16 lanes a row, 8 channels a lane (D <= 128)
+template <typename T> __global__ void __launch_bounds__(256) mha_delta_kernel(const MhaParams P) {
+  const long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4), n = (long long)P.B * P.Hq * P.Tq;
+  if (i >= n) return;
+  const int c = (threadIdx.x & 15) * 8, tq = (int)(i % P.Tq), hq = (int)(i / P.Tq % P.Hq), b = (int)(i / P.Tq / P.Hq);
+  const int lq = mh_len(P.q_len, b, P.Tq);
+  float s = 0.f;
+  if (tq < lq && c < P.D) {
+    float x[8], y[8];
+    const long long at = b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh;
+    mh_load8((const T*)P.o + at, c, P.D, x);
+    mh_load8((const T*)P.d_o + at, c, P.D, y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += x[j] * y[j];
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 15) == 0) P.delta[i] = s;
+}
+
+// accumulators (channels on rows, this lane's token on the column) -> row of a tensor, or fp32 partial row
+template <typename T, int DB> __device__ __forceinline__ void mh_put(const mh_f32x16 (&a)[DB], float f, bool keep, T* row, int D, int h) {
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = d * 32 + g * 8 + h * 4;
+      mh_store4<T>(row, c, D, keep ? a[d][g * 4] * f : 0.f, keep ? a[d][g * 4 + 1] * f : 0.f, keep ? a[d][g * 4 + 2] * f : 0.f, keep ? a[d][g * 4 + 3] * f : 0.f);
+    }
+}
+
+template <typename T, int DP, int KT, int OCC>
+__global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
+  constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, KB = KT / 32;
+  constexpr int TE = MhTile<NP, KT, DP>::ELEMS;
+  extern __shared__ __attribute__((aligned(16))) unsigned short mh_sm[];       // [2 buffers][K tile | V tile]
+  int unit, tile, split;
+  if (!mh_where(P, unit, tile, split)) return;
+  if (P.causal) tile = P.tiles - 1 - tile;
+  const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), li = lane & 31, h = lane >> 5;
+  const int b = unit / P.Hq, hq = unit % P.Hq, hk = hq / P.G;
+  const int lq = mh_len(P.q_len, b, P.Tq), lk = mh_len(P.k_len, b, P.Tk), off = lk - lq;
+  const int row0 = tile * 128, tq = row0 + wv * 32 + li;
+  const T* kbase = (const T*)P.k + b * P.kb + hk * P.kh;
+  const T* vbase = (const T*)P.v + b * P.vb + hk * P.vh;
+  int nk = row0 >= lq ? 0 : P.causal ? min(lk, min(row0 + 127, lq - 1) + off + 1) : lk;
+  nk = max(nk, 0);
+  const int ntiles = (nk + KT - 1) / KT;
+  const int tb = (int)((long long)ntiles * split / P.splits), te = (int)((long long)ntiles * (split + 1) / P.splits);
+  const bool ok = tq < lq && lk > 0 && (!P.causal || tq + off >= 0);           // the query exists and sees a key
+  const int kmax = ok ? (P.causal ? min(lk, tq + off + 1) : lk) : lk;
+  const bool wlive = __any(ok);
+
+  mh_bf16x8 Q[KS][NP], G[KS][NP];
+  mh_row_frags<T, NP, DP>((const T*)P.q + b * P.qb + (long long)tq * P.qt + (long long)hq * P.qh, ok, P.D, h, Q);
+  mh_row_frags<T, NP, DP>((const T*)P.d_o + b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh, ok, P.D, h, G);
+  float lse2 = MH_INF, del = 0.f;
+  if (ok) {
+    const long long i = ((long long)b * P.Hq + hq) * P.Tq + tq;
+    const float e = P.lse[i];
+    lse2 = e == -MH_INF ? MH_INF : e * MH_LOG2E;
+    del = P.delta[i];
+  }
+  mh_f32x16 dQ[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) mh_zero(dQ[d]);
+
+  MhStage<T, NP, KT, DP> sk, sv;
+  if (tb < te) {
+    sk.load(kbase, P.kt, tb * KT, 0, lk, P.D);
+    sv.load(vbase, P.vt, tb * KT, 0, lk, P.D);
+    sk.store(mh_sm); sv.store(mh_sm + TE);
+  }
+  __syncthreads();
+  for (int it = tb; it < te; ++it) {
+    const unsigned short* cur = mh_sm + ((it - tb) & 1) * 2 * TE;
+    unsigned short* nxt = mh_sm + (((it - tb) & 1) ^ 1) * 2 * TE;
+    const bool more = it + 1 < te;
+    if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk, P.D); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk, P.D); }
+    const int k0 = it * KT;
+    if (wlive && __any(kmax > k0)) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        mh_f32x16 S, E;
+        mh_zero(S); mh_zero(E);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          mh_bf16x8 A[NP];
+          mh_frag_rows<NP, KT, DP>(cur, kb * 32, ks, li, h, A);
+          mh_mma<NP>(A, Q[ks], S);
+          mh_frag_rows<NP, KT, DP>(cur + TE, kb * 32, ks, li, h, A);
+          mh_mma<NP>(A, G[ks], E);
+        }
+        const int base = k0 + kb * 32 + 4 * h;
+        const bool cut = __any(k0 + kb * 32 + 32 > kmax);
+        mh_bf16x8 F[2][NP];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int r = s * 8 + j;
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], P.sc2, -lse2));
+            e[j] = p * (E[r] - del);
+            if (cut && base + (r & 3) + 8 * (r >> 2) >= kmax) e[j] = 0.f;
+          }
+          mh_planes<NP>(e, F[s]);
+        }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            mh_bf16x8 A[NP];
+            mh_frag_cols<NP, KT, DP>(cur, kb * 32 + s * 16, d, lane, A);
+            mh_mma<NP>(A, F[s], dQ[d]);
+          }
+      }
+    }
+    if (more) { sk.store(nxt); sv.store(nxt + TE); }
+    __syncthreads();
+  }
+  if (tq >= P.Tq) return;
+  if (P.splits > 1) {
+    float* row = P.part + (((long long)split * P.B * P.Hq + unit) * P.Tq + tq) * P.D;
+    mh_put<float, DB>(dQ, P.scale, ok, row, P.D, h);
+  } else {
+    mh_put<T, DB>(dQ, P.scale, ok, (T*)P.dq + b * P.qb + (long long)tq * P.qt + (long long)hq * P.qh, P.D, h);
+  }
+}
+
+template <typename T, int DP, int QT, int OCC>
+__global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
+  constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, QB = QT / 32;
+  constexpr int TE = MhTile<NP, QT, DP>::ELEMS, BUF = 2 * TE + 4 * QT;         // Q tile | dO tile | lse2[QT], delta[QT] (floats)
+  extern __shared__ __attribute__((aligned(16))) unsigned short mh_sm[];
+  int unit, tile, split;
+  if (!mh_where(P, unit, tile, split)) return;
+  const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), li = lane & 31, h = lane >> 5;
+  const int b = unit / P.Hkv, hk = unit % P.Hkv;
+  const int lq = mh_len(P.q_len, b, P.Tq), lk = mh_len(P.k_len, b, P.Tk), off = lk - lq;
+  const int key0 = tile * 128, kw = key0 + wv * 32, key = kw + li;
+  const bool ok = key < lk;
+  const int qlo = P.causal ? max(0, -off) : 0;                                 // first query that sees a key
+  const int first = P.causal ? max(qlo, key0 - off) : 0;                       // first query that sees key0
+  const int q0t = first / QT, nq = key0 < lk && first < lq ? (lq + QT - 1) / QT - q0t : 0;
+  const long long items = (long long)nq * P.G;
+  const long long ib = items * split / P.splits, ie = items * (split + 1) / P.splits;
+
+  mh_bf16x8 K[KS][NP], V[KS][NP];
+  mh_row_frags<T, NP, DP>((const T*)P.k + b * P.kb + (long long)key * P.kt + (long long)hk * P.kh, ok, P.D, h, K);
+  mh_row_frags<T, NP, DP>((const T*)P.v + b * P.vb + (long long)key * P.vt + (long long)hk * P.vh, ok, P.D, h, V);
+  mh_f32x16 dK[DB], dV[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) { mh_zero(dK[d]); mh_zero(dV[d]); }
+
+  MhStage<T, NP, QT, DP> sq, sg;
+  float rl = 0.f, rd = 0.f;
+  auto load = [&](long long it) {
+    const int hq = hk * P.G + (int)(it / nq), q0 = (q0t + (int)(it % nq)) * QT;
+    sq.load((const T*)P.q + b * P.qb + (long long)hq * P.qh, P.qt, q0, qlo, lq, P.D);
+    sg.load((const T*)P.d_o + b * P.ob + (long long)hq * P.oh, P.ot, q0, qlo, lq, P.D);
+    if (t < QT) {
+      const int tq = q0 + t;
+      rl = MH_INF; rd = 0.f;
+      if (tq >= qlo && tq < lq) {
+        const long long i = ((long long)b * P.Hq + hq) * P.Tq + tq;
+        const float e = P.lse[i];
+        rl = e == -MH_INF ? MH_INF : e * MH_LOG2E;
+        rd = P.delta[i];
+      }
+    }
+  };
+  auto store = [&](unsigned short* buf) {
+    sq.store(buf); sg.store(buf + TE);
+    float* st = reinterpret_cast<float*>(buf + 2 * TE);
+    if (t < QT) { st[t] = rl; st[QT + t] = rd; }
+  };
+  if (ib < ie) { load(ib); store(mh_sm); }
+  __syncthreads();
+  for (long long it = ib; it < ie; ++it) {
+    const unsigned short* cur = mh_sm + ((it - ib) & 1) * BUF;
+    unsigned short* nxt = mh_sm + (((it - ib) & 1) ^ 1) * BUF;
+    const bool more = it + 1 < ie;
+    if (more) load(it + 1);
+    const int q0 = (q0t + (int)(it % nq)) * QT;
+    const float* st = reinterpret_cast<const float*>(cur + 2 * TE);
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      const int qa = q0 + qb * 32;
+      if (kw >= lk || (P.causal && qa + 31 + off < kw)) continue;              // no pair of this wave (uniform)
+      mh_f32x16 S, E;
+      mh_zero(S); mh_zero(E);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        mh_bf16x8 A[NP];
+        mh_frag_rows<NP, QT, DP>(cur, qb * 32, ks, li, h, A);
+        mh_mma<NP>(A, K[ks], S);
+        mh_frag_rows<NP, QT, DP>(cur + TE, qb * 32, ks, li, h, A);
+        mh_mma<NP>(A, V[ks], E);
+      }
+      const bool cut = P.causal && qa + off < kw + 31;
+      mh_bf16x8 FP[2][NP], FS[2][NP];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float p[8], e[8];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {                                          // four consecutive queries: rows 8 (2 s + g) + 4 h ..+3
+          const tk_f32x4 l4 = *reinterpret_cast<const tk_f32x4*>(st + qb * 32 + 8 * (2 * s + g) + 4 * h);
+          const tk_f32x4 d4 = *reinterpret_cast<const tk_f32x4*>(st + QT + qb * 32 + 8 * (2 * s + g) + 4 * h);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = s * 8 + g * 4 + j;
+            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], P.sc2, -l4[j]));
+            float y = x * (E[r] - d4[j]);
+            if (cut && qa + 8 * (2 * s + g) + 4 * h + j + off < key) { x = 0.f; y = 0.f; }
+            p[g * 4 + j] = x; e[g * 4 + j] = y;
+          }
+        }
+        mh_planes<NP>(p, FP[s]);
+        mh_planes<NP>(e, FS[s]);
+      }
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          mh_bf16x8 A[NP];
+          mh_frag_cols<NP, QT, DP>(cur + TE, qb * 32 + s * 16, d, lane, A);
+          mh_mma<NP>(A, FP[s], dV[d]);
+          mh_frag_cols<NP, QT, DP>(cur, qb * 32 + s * 16, d, lane, A);
+          mh_mma<NP>(A, FS[s], dK[d]);
+        }
+    }
+    if (more) store(nxt);
+    __syncthreads();
+  }
+  if (key >= P.Tk) return;
+  if (P.splits > 1) {
+    const long long n = (long long)P.B * P.Hkv * P.Tk;
+    float* row = P.part + ((long long)split * 2 * n + (long long)unit * P.Tk + key) * P.D;
+    mh_put<float, DB>(dK, P.scale, ok, row, P.D, h);
+    mh_put<float, DB>(dV, 1.f, ok, row + n * P.D, P.D, h);
+  } else {
+    mh_put<T, DB>(dK, P.scale, ok, (T*)P.dk + b * P.kb + (long long)key * P.kt + (long long)hk * P.kh, P.D, h);
+    mh_put<T, DB>(dV, 1.f, ok, (T*)P.dv + b * P.vb + (long long)key * P.vt + (long long)hk * P.vh, P.D, h);
+  }
+}
+
+// out[b][t][h][d] = sum over splits of part[s][(b, h, t)][d], in order; `step`: floats between two ranges
+template <typename T>
+__global__ void __launch_bounds__(256) mha_bwd_join_kernel(const float* __restrict__ part, long long step, int splits, T* out, long long sb, long long stt, long long sh,
+                                                           int H, int Tn, int D, long long n) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+  for (int k = 0; k < splits; ++k) s += part[k * step + i];
+  const int d = (int)(i % D);
+  const long long row = i / D;
+  const int tok = (int)(row % Tn), hh = (int)(row / Tn % H), b = (int)(row / Tn / H);
+  TkVec<T>::store(out + b * sb + (long long)tok * stt + (long long)hh * sh + d, s);
+}
+
+// ---- host
+// Ranges of the summed axis when the tiles alone give fewer than two workgroups a CU; at least 4 tiles of the summed axis a range.
+static int mh_bwd_splits(long long wgs, long long axis_tiles) {
+  if (wgs <= 0) return 1;
+  long long s = (512 + wgs - 1) / wgs;
+  if (s > axis_tiles / 4) s = axis_tiles / 4;
+  return s < 1 ? 1 : (int)s;
+}
+struct MhaBwdPlan { int dq_tiles, dq_splits, dkv_tiles, dkv_splits; size_t delta_floats, dq_floats, dkv_floats; };
+static MhaBwdPlan mh_bwd_plan(const MhaParams& P) {
+  MhaBwdPlan L = {};
+  L.delta_floats = ((size_t)P.B * P.Hq * P.Tq + 3) / 4 * 4;
+  if (P.Tq > 0) {
+    L.dq_tiles = cdiv(P.Tq, 128);
+    L.dq_splits = mh_bwd_splits((long long)L.dq_tiles * P.B * P.Hq, cdiv(P.Tk, 64));
+    if (L.dq_splits > 1) L.dq_floats = (size_t)L.dq_splits * P.B * P.Hq * P.Tq * P.D;
+  }
+  if (P.Tk > 0) {
+    L.dkv_tiles = cdiv(P.Tk, 128);
+    L.dkv_splits = mh_bwd_splits((long long)L.dkv_tiles * P.B * P.Hkv, (long long)cdiv(P.Tq, 32) * P.G);
+    if (L.dkv_splits > 1) L.dkv_floats = (size_t)L.dkv_splits * 2 * P.B * P.Hkv * P.Tk * P.D;
+  }
+  return L;
+}
+size_t k_mha_bwd_workspace_bytes(const MhaParams& P) {
+  const MhaBwdPlan L = mh_bwd_plan(P);                                         // dQ and dK / dV partials share their space: the kernels run one after the other
+  return (L.delta_floats + (L.dq_floats > L.dkv_floats ? L.dq_floats : L.dkv_floats)) * sizeof(float);
+}
+
+template <typename T, int DP, int KT, int OCC> static void mh_dq_go(const MhaParams& P, hipStream_t st) {
+  constexpr int lds = 4 * MhTile<MhNP<T>::NP, KT, DP>::ELEMS * 2;
+  static_assert(lds <= 163840, "LDS");
+  hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_dq_kernel<T, DP, KT, OCC>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL((mha_dq_kernel<T, DP, KT, OCC>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
+}
+template <typename T, int DP, int QT, int OCC> static void mh_dkv_go(const MhaParams& P, hipStream_t st) {
+  constexpr int lds = 2 * (2 * MhTile<MhNP<T>::NP, QT, DP>::ELEMS + 4 * QT) * 2;
+  static_assert(lds <= 163840, "LDS");
+  hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_dkv_kernel<T, DP, QT, OCC>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL((mha_dkv_kernel<T, DP, QT, OCC>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
+}
+template <typename T> static void mh_bwd_join(const float* part, long long step, int splits, void* out, long long sb, long long stt, long long sh, int H, int Tn, int D,
+                                              long long rows, hipStream_t st) {
+  const long long n = rows * D;
+  hipLaunchKernelGGL((mha_bwd_join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, step, splits, (T*)out, sb, stt, sh, H, Tn, D, n);
+}
+
+int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStream_t st) {
+  MhaParams P = P0;
+  const bool bf = dtype == PDAE_DT_BF16;
+  const MhaBwdPlan L = mh_bwd_plan(P);
+  const size_t need = k_mha_bwd_workspace_bytes(P);
+  if (P.B == 0 || (P.Tq == 0 && P.Tk == 0)) return PDAE_OK;
+  PDAE_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "mha_bwd: needs %zu bytes of workspace (got %zu)", need, ws ? ws_bytes : (size_t)0);
+  P.delta = (float*)ws;
+  P.part = (float*)ws + L.delta_floats;
+  const long long nq = (long long)P.B * P.Hq * P.Tq, nk = (long long)P.B * P.Hkv * P.Tk;
+  PDAE_CHECK_ARG(nq * P.D / 256 < (1ll << 31) && nk * P.D / 256 < (1ll << 31), "mha_bwd: too many rows for one launch");
+  if (P.Tq > 0) {
+    if (bf) hipLaunchKernelGGL((mha_delta_kernel<tk_bf16>), dim3(cdiv(nq, 16)), dim3(256), 0, st, P);
+    else hipLaunchKernelGGL((mha_delta_kernel<float>), dim3(cdiv(nq, 16)), dim3(256), 0, st, P);
+    P.units = P.B * P.Hq; P.tiles = L.dq_tiles; P.splits = L.dq_splits;
+    PDAE_CHECK_ARG(mh_grid(P) < (1ll << 31), "mha_bwd: too many query tiles for one launch");
+    if (bf) {
+      if (P.D <= 32) mh_dq_go<tk_bf16, 32, 64, 2>(P, st);
+      else if (P.D <= 64) mh_dq_go<tk_bf16, 64, 64, 2>(P, st);
+      else if (P.D <= 96) mh_dq_go<tk_bf16, 96, 64, 2>(P, st);
+      else mh_dq_go<tk_bf16, 128, 64, 1>(P, st);
+    } else {
+      if (P.D <= 32) mh_dq_go<float, 32, 32, 2>(P, st);
+      else if (P.D <= 64) mh_dq_go<float, 64, 32, 2>(P, st);
+      else if (P.D <= 96) mh_dq_go<float, 96, 32, 1>(P, st);
+      else mh_dq_go<float, 128, 32, 1>(P, st);
+    }
+    if (int e = pdae_launch_status("mha_dq")) return e;
+    if (P.splits > 1) {
+      if (bf) mh_bwd_join<tk_bf16>(P.part, nq * P.D, P.splits, P.dq, P.qb, P.qt, P.qh, P.Hq, P.Tq, P.D, nq, st);
+      else mh_bwd_join<float>(P.part, nq * P.D, P.splits, P.dq, P.qb, P.qt, P.qh, P.Hq, P.Tq, P.D, nq, st);
+    }
+  }
+  if (P.Tk > 0) {
+    P.units = P.B * P.Hkv; P.tiles = L.dkv_tiles; P.splits = L.dkv_splits;
+    PDAE_CHECK_ARG(mh_grid(P) < (1ll << 31), "mha_bwd: too many key tiles for one launch");
+    if (bf) {
+      if (P.D <= 32) mh_dkv_go<tk_bf16, 32, 32, 2>(P, st);
+      else if (P.D <= 64) mh_dkv_go<tk_bf16, 64, 32, 2>(P, st);
+      else if (P.D <= 96) mh_dkv_go<tk_bf16, 96, 32, 1>(P, st);
+      else mh_dkv_go<tk_bf16, 128, 32, 1>(P, st);
+    } else {
+      if (P.D <= 32) mh_dkv_go<float, 32, 32, 2>(P, st);
+      else if (P.D <= 64) mh_dkv_go<float, 64, 32, 1>(P, st);
+      else if (P.D <= 96) mh_dkv_go<float, 96, 32, 1>(P, st);
+      else mh_dkv_go<float, 128, 32, 1>(P, st);
+    }
+    if (int e = pdae_launch_status("mha_dkv")) return e;
+    if (P.splits > 1) {
+      const long long step = 2 * nk * P.D;
+      if (bf) {
+        mh_bwd_join<tk_bf16>(P.part, step, P.splits, P.dk, P.kb, P.kt, P.kh, P.Hkv, P.Tk, P.D, nk, st);
+        mh_bwd_join<tk_bf16>(P.part + nk * P.D, step, P.splits, P.dv, P.vb, P.vt, P.vh, P.Hkv, P.Tk, P.D, nk, st);
+      } else {
+        mh_bwd_join<float>(P.part, step, P.splits, P.dk, P.kb, P.kt, P.kh, P.Hkv, P.Tk, P.D, nk, st);
+        mh_bwd_join<float>(P.part + nk * P.D, step, P.splits, P.dv, P.vb, P.vt, P.vh, P.Hkv, P.Tk, P.D, nk, st);
+      }
+    }
+  }
+  return pdae_launch_status("mha_bwd");
+}

@@ -1,0 +1,265 @@
+// Attention forward for any number of tokens (mha.h): one pass over the keys with a running maximum and sum per query.
+//
+// Workgroup = 4 waves; wave w owns QB * 32 query rows (its Q fragments stay in registers), the four share key / value tiles of KT tokens in LDS, double
+// buffered: the next tile travels from HBM into registers while this one is multiplied, and is stored to the other buffer behind it: one barrier per tile.
+// Per 32 keys x 32 queries: S^T = K Q^T (DP / 16 MFMAs), t = sc2 s, running maximum m in the log2 domain, p = 2^(t - m), O^T += V^T P (DP / 16 MFMAs).
+// Every lane holds 16 of a column's 32 scores: the row maximum is a register tree and one exchange with lane ^ 32, the sum stays per lane until the end.
+//
+// Few rows (a token or a few per sample against a long cache): query heads that share a key head are rows of ONE tile (GP = G), and the keys are split into
+// ranges (grid `splits`), each leaving an unnormalised partial (O, m, l); mha_join_kernel adds them in a fixed order.
+#include "kernels.h"
+#include "mha.h"
+
+template <typename T, int DP, int QB, int KT, int OCC>
+__global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
+  constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, KB = KT / 32;
+  constexpr int TE = MhTile<NP, KT, DP>::ELEMS;
+  extern __shared__ __attribute__((aligned(16))) unsigned short mh_sm[];       // [2 buffers][K tile | V tile]
+  int unit, tile, split;
+  if (!mh_where(P, unit, tile, split)) return;
+  if (P.causal) tile = P.tiles - 1 - tile;                                     // long rows first
+  const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), li = lane & 31, h = lane >> 5;
+  const int b = unit / P.HP, hp = unit % P.HP, hk = hp * P.GP / P.G;
+  const int lq = mh_len(P.q_len, b, P.Tq), lk = mh_len(P.k_len, b, P.Tk), off = lk - lq;
+  const int row0 = tile * (128 * QB);
+  const T* kbase = (const T*)P.k + b * P.kb + hk * P.kh;
+  const T* vbase = (const T*)P.v + b * P.vb + hk * P.vh;
+
+  // keys the tile's last existing query sees
+  int tlast = (min(row0 + 128 * QB, P.R) - 1) / P.GP;
+  tlast = min(tlast, lq - 1);
+  int nk = row0 / P.GP >= lq ? 0 : P.causal ? min(lk, tlast + off + 1) : lk;
+  nk = max(nk, 0);
+  const int ntiles = (nk + KT - 1) / KT;
+  const int tb = (int)((long long)ntiles * split / P.splits), te = (int)((long long)ntiles * (split + 1) / P.splits);
+
+  // this lane's query columns
+  mh_bf16x8 Q[QB][KS][NP];
+  int kmax[QB], qrow[QB];
+  bool live = false;
+#pragma unroll
+  for (int a = 0; a < QB; ++a) {
+    const int r = row0 + wv * (32 * QB) + a * 32 + li, tq = r / P.GP, hq = hp * P.GP + r % P.GP;
+    qrow[a] = r;
+    const bool ok = r < P.R && tq < lq;
+    kmax[a] = ok ? (P.causal ? min(lk, tq + off + 1) : lk) : lk;               // rows that do not exist never force the masked path; they are zeroed at the end
+    live = live || ok;
+    mh_row_frags<T, NP, DP>((const T*)P.q + b * P.qb + (long long)tq * P.qt + (long long)hq * P.qh, ok, P.D, h, Q[a]);
+  }
+  const bool wlive = __any(live);
+  int kwave = 0;                                                               // last key any of the wave's rows sees
+#pragma unroll
+  for (int a = 0; a < QB; ++a) kwave = max(kwave, kmax[a]);
+
+  mh_f32x16 O[QB][DB];
+  float m[QB], l[QB];
+#pragma unroll
+  for (int a = 0; a < QB; ++a) {
+    m[a] = -MH_INF; l[a] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) mh_zero(O[a][d]);
+  }
+
+  MhStage<T, NP, KT, DP> sk, sv;
+  if (tb < te) {
+    sk.load(kbase, P.kt, tb * KT, 0, lk, P.D);
+    sv.load(vbase, P.vt, tb * KT, 0, lk, P.D);
+    sk.store(mh_sm); sv.store(mh_sm + TE);
+  }
+  __syncthreads();
+  for (int it = tb; it < te; ++it) {
+    const unsigned short* cur = mh_sm + ((it - tb) & 1) * 2 * TE;
+    unsigned short* nxt = mh_sm + (((it - tb) & 1) ^ 1) * 2 * TE;
+    const bool more = it + 1 < te;
+    if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk, P.D); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk, P.D); }
+    const int k0 = it * KT;
+    if (wlive && __any(kwave > k0)) {
+      mh_f32x16 S[QB][KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+        for (int a = 0; a < QB; ++a) mh_zero(S[a][kb]);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          mh_bf16x8 A[NP];
+          mh_frag_rows<NP, KT, DP>(cur, kb * 32, ks, li, h, A);
+#pragma unroll
+          for (int a = 0; a < QB; ++a) mh_mma<NP>(A, Q[a][ks], S[a][kb]);
+        }
+      }
+      mh_bf16x8 F[QB][KB][2][NP];
+#pragma unroll
+      for (int a = 0; a < QB; ++a) {
+        if (__any(k0 + KT > kmax[a])) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) mh_mask_keys(S[a][kb], k0 + kb * 32 + 4 * h, kmax[a]);
+        }
+        float mx = S[a][0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[a][kb][r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float mn = fmaxf(m[a], mx * P.sc2), ms = mn == -MH_INF ? 0.f : mn;      // a column that has seen no key yet keeps p = 2^-inf = 0
+        const float al = __builtin_amdgcn_exp2f(m[a] - ms);
+        m[a] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[a][kb][s * 8 + j], P.sc2, -ms)); sum += e[j]; }
+            mh_planes<NP>(e, F[a][kb][s]);
+          }
+        l[a] = l[a] * al + sum;
+        if (__any(al != 1.f)) {
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) O[a][d][r] *= al;
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            mh_bf16x8 A[NP];
+            mh_frag_cols<NP, KT, DP>(cur + TE, kb * 32 + s * 16, d, lane, A);
+#pragma unroll
+            for (int a = 0; a < QB; ++a) mh_mma<NP>(A, F[a][kb][s], O[a][d]);
+          }
+    }
+    if (more) { sk.store(nxt); sv.store(nxt + TE); }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int a = 0; a < QB; ++a) {
+    const int r = qrow[a];
+    if (r >= P.R) continue;
+    const int tq = r / P.GP, hq = hp * P.GP + r % P.GP;
+    const float ls = l[a] + __shfl_xor(l[a], 32);
+    if (P.splits > 1) {
+      const long long idx = ((long long)split * P.units + unit) * P.R + r;
+      float* po = P.part + idx * P.D;
+      float* ml = P.part + (long long)P.splits * P.units * P.R * P.D + idx * 2;
+      const bool any = tq < lq && ls != 0.f;                                   // (NaN counts: it has to reach the output)
+      if (h == 0) { ml[0] = any ? m[a] : -MH_INF; ml[1] = any ? ls : 0.f; }
+      if (any) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) mh_store4<float>(po, d * 32 + g * 8 + h * 4, P.D, O[a][d][g * 4], O[a][d][g * 4 + 1], O[a][d][g * 4 + 2], O[a][d][g * 4 + 3]);
+      }
+      continue;
+    }
+    const bool any = tq < lq && ls != 0.f;                                     // padded rows and rows whose masks leave nothing: zero
+    const float inv = any ? 1.0f / ls : 0.f;
+    T* orow = (T*)P.out + b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float x0 = any ? O[a][d][g * 4] * inv : 0.f, x1 = any ? O[a][d][g * 4 + 1] * inv : 0.f;
+        const float x2 = any ? O[a][d][g * 4 + 2] * inv : 0.f, x3 = any ? O[a][d][g * 4 + 3] * inv : 0.f;
+        mh_store4<T>(orow, d * 32 + g * 8 + h * 4, P.D, x0, x1, x2, x3);
+      }
+    if (P.lse && h == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = any ? (m[a] + __builtin_amdgcn_logf(ls)) * MH_LN2 : -MH_INF;      // (v_log_f32: log2)
+  }
+}
+
+// Adds the key ranges of a split forward: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  One wave per row.
+template <typename T>
+__global__ void __launch_bounds__(256) mha_join_kernel(const MhaParams P) {
+  const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), n = (long long)P.units * P.R;
+  if (i >= n) return;
+  const int lane = threadIdx.x & 63, unit = (int)(i / P.R), r = (int)(i % P.R), b = unit / P.HP, hq = unit % P.HP * P.GP + r % P.GP, tq = r / P.GP;
+  const float* ml = P.part + (long long)P.splits * n * P.D;
+  float M = -MH_INF;
+  for (int s = 0; s < P.splits; ++s) { const float* e = ml + (s * n + i) * 2; if (e[1] != 0.f) M = fmaxf(M, e[0]); }
+  const float Ms = M == -MH_INF ? 0.f : M;
+  float L = 0.f, o0 = 0.f, o1 = 0.f;
+  const int c = lane * 2;
+  for (int s = 0; s < P.splits; ++s) {
+    const float* e = ml + (s * n + i) * 2;
+    const float ls = e[1];
+    if (ls == 0.f) continue;                                                   // an empty range wrote no O
+    const float w = __builtin_amdgcn_exp2f(e[0] - Ms);
+    const float* po = P.part + (s * n + i) * P.D;
+    L += w * ls;
+    if (c < P.D) o0 += w * po[c];
+    if (c + 1 < P.D) o1 += w * po[c + 1];
+  }
+  const float inv = L != 0.f ? 1.0f / L : 0.f;
+  T* orow = (T*)P.out + b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh;
+  if (c < P.D) TkVec<T>::store(orow + c, L != 0.f ? o0 * inv : 0.f);
+  if (c + 1 < P.D) TkVec<T>::store(orow + c + 1, L != 0.f ? o1 * inv : 0.f);
+  if (P.lse && lane == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * MH_LN2 : -MH_INF;
+}
+
+// ---- host: row packing, key ranges
+static int mh_qb(int dtype, int R, int D) { return dtype == PDAE_DT_BF16 && R > 128 && D <= 64 ? 2 : 1; }
+// Rows of a tile: with few query tokens the G heads that share a key head become rows of one tile, so its keys are read once for all of them.
+// Then, when the tiles alone do not give every CU two workgroups, the keys are split into ranges of at least 256.
+static void mh_fwd_plan(MhaParams& P, int dtype) {
+  P.GP = (long long)P.Tq * P.G <= 128 ? P.G : 1;
+  P.HP = P.Hq / P.GP;
+  P.R = P.Tq * P.GP;
+  P.units = P.B * P.HP;
+  P.tiles = cdiv(P.R, 128 * mh_qb(dtype, P.R, P.D));
+  const long long wgs = (long long)P.units * P.tiles;
+  long long s = (512 + wgs - 1) / wgs;
+  const long long most = P.Tk / 256;
+  if (s > most) s = most;
+  P.splits = s < 1 ? 1 : (int)s;
+}
+static size_t mh_fwd_part_floats(const MhaParams& P) { return P.splits > 1 ? (size_t)P.splits * P.units * P.R * (P.D + 2) : 0; }
+
+size_t k_mha_fwd_workspace_bytes(const MhaParams& P0, int dtype) {
+  MhaParams P = P0;
+  if (P.B <= 0 || P.Tq <= 0) return 0;
+  mh_fwd_plan(P, dtype);
+  return mh_fwd_part_floats(P) * sizeof(float);
+}
+
+template <typename T, int DP, int QB, int KT, int OCC> static void mh_fwd_go(const MhaParams& P, hipStream_t st) {
+  constexpr int NP = MhNP<T>::NP;
+  const size_t lds = (size_t)4 * MhTile<NP, KT, DP>::ELEMS * 2;
+  static_assert(4 * MhTile<NP, KT, DP>::ELEMS * 2 <= 163840, "LDS");
+  hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_fwd_kernel<T, DP, QB, KT, OCC>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  hipLaunchKernelGGL((mha_fwd_kernel<T, DP, QB, KT, OCC>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
+}
+
+int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStream_t st) {
+  MhaParams P = P0;
+  if (P.B == 0 || P.Tq == 0) return PDAE_OK;
+  mh_fwd_plan(P, dtype);
+  const size_t need = mh_fwd_part_floats(P) * sizeof(float);
+  PDAE_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "mha_fwd: needs %zu bytes of workspace (got %zu)", need, ws ? ws_bytes : (size_t)0);
+  PDAE_CHECK_ARG(mh_grid(P) < (1ll << 31) && (long long)P.units * P.R < (1ll << 31), "mha_fwd: too many query rows for one launch");
+  P.part = (float*)ws;
+  const int qb = mh_qb(dtype, P.R, P.D);
+  if (dtype == PDAE_DT_BF16) {
+    if (P.D <= 32) { if (qb == 2) mh_fwd_go<tk_bf16, 32, 2, 64, 2>(P, st); else mh_fwd_go<tk_bf16, 32, 1, 64, 2>(P, st); }
+    else if (P.D <= 64) { if (qb == 2) mh_fwd_go<tk_bf16, 64, 2, 64, 2>(P, st); else mh_fwd_go<tk_bf16, 64, 1, 64, 2>(P, st); }
+    else if (P.D <= 96) mh_fwd_go<tk_bf16, 96, 1, 64, 2>(P, st);
+    else mh_fwd_go<tk_bf16, 128, 1, 64, 2>(P, st);
+  } else {
+    if (P.D <= 32) mh_fwd_go<float, 32, 1, 32, 2>(P, st);
+    else if (P.D <= 64) mh_fwd_go<float, 64, 1, 32, 2>(P, st);
+    else if (P.D <= 96) mh_fwd_go<float, 96, 1, 32, 1>(P, st);
+    else mh_fwd_go<float, 128, 1, 32, 1>(P, st);
+  }
+  if (int e = pdae_launch_status("mha_fwd")) return e;
+  if (P.splits > 1) {
+    const long long n = (long long)P.units * P.R;
+    if (dtype == PDAE_DT_BF16) hipLaunchKernelGGL((mha_join_kernel<tk_bf16>), dim3(cdiv(n, 4)), dim3(256), 0, st, P);
+    else hipLaunchKernelGGL((mha_join_kernel<float>), dim3(cdiv(n, 4)), dim3(256), 0, st, P);
+    return pdae_launch_status("mha_join");
+  }
+  return PDAE_OK;
+}

@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get("PDAE_HIP_LIB") or os.path.join(_HERE, "lib", "libpdae
  OP_SILU_BWD, OP_AXPBY, OP_EMBEDDING, OP_EMBEDDING_BWD, OP_TO_NHWC, OP_FROM_NHWC, OP_Q_SAMPLE, OP_LOSS, OP_DDIM_STEP,
  OP_DDPM_STEP, OP_ADAM_EMA, OP_SOFTMAX, OP_SOFTMAX_BWD, OP_COLSUM, OP_MEMSET, OP_COPY, OP_CONV_WPREP, OP_MLP_MODLN_FWD, OP_MLP_MODLN_BWD, OP_CONV_FWD_GN, OP_CONV_FWD_SKIP, OP_GN_STATS_COEF, OP_CONV_SKIP_WPREP, OP_AMAX,
  OP_AXPBY_ROWS, OP_DDIM_STEP_ROWS, OP_DDPM_STEP_ROWS, OP_LINEAR_GROUP, OP_ATTN_FWD, OP_ATTN_BWD, OP_LINEAR_BWD_GROUP, OP_GN_COEF_FROM_CONV_STATS, OP_CONV_WPREP_GROUP, OP_SUBSAMPLE2,
- OP_ZERO_INSERT2, OP_GN_STATS_QUADS, OP_JOIN) = range(1, 48)
+ OP_ZERO_INSERT2, OP_GN_STATS_QUADS, OP_JOIN, OP_LAYERNORM_FWD, OP_LAYERNORM_BWD, OP_DROPOUT_FWD, OP_DROPOUT_BWD, OP_MHA_FWD, OP_MHA_BWD) = range(1, 54)
 OPF_SIDE = 1            # PdaeOp.flags: issue on the executor's second stream (pdae_hip.h)
 
 
@@ -25,9 +25,19 @@ class PdaeOp(ctypes.Structure):
                 ("i", ctypes.c_int64 * 24), ("f", ctypes.c_double * 12)]
 
 
+DT_F32, DT_BF16 = 0, 1                                            # PDAE_F32 / PDAE_BF16: element type of the token operators
+DTYPES = {"f32": DT_F32, "bf16": DT_BF16, torch.float32: DT_F32, torch.bfloat16: DT_BF16}
+
+
 class ConvDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in
                 ("N", "Hi", "Wi", "C0", "C1", "Ho", "Wo", "Cout", "KH", "KW", "stride", "pad", "up", "math")]
+
+
+class MhaDesc(ctypes.Structure):
+    """pdae_mha_desc (include/pdae_hip.h)."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "Tq", "Tk", "Hq", "Hkv", "D", "dtype", "causal")] + \
+               [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + [("scale", ctypes.c_float)]
 
 
 MATH_F32, MATH_BF16, MATH_BF16X3, MATH_BF16X6 = 0, 1, 2, 3      # pdae_conv_desc.math
@@ -101,6 +111,10 @@ def lib():
         L.pdae_image_prepare.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 9 + [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
                                                                                  ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64),
                                                                                  ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+        L.pdae_layernorm_workspace_bytes.argtypes = [ctypes.c_int, ctypes.c_int]
+        L.pdae_layernorm_workspace_bytes.restype = ctypes.c_size_t
+        L.pdae_mha_workspace_bytes.argtypes = [ctypes.POINTER(MhaDesc), ctypes.c_int]
+        L.pdae_mha_workspace_bytes.restype = ctypes.c_size_t
         L.pdae_set_knob.argtypes = [ctypes.c_char_p, ctypes.c_int]
         L.pdae_set_knob.restype = ctypes.c_int
         L.pdae_get_knob.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int)]
@@ -116,7 +130,9 @@ EXPORTS = ["pdae_last_error", "pdae_abi_version", "pdae_set_knob", "pdae_get_kno
            "pdae_mlp_modln_fwd", "pdae_mlp_modln_bwd", "pdae_timestep_embedding", "pdae_amax", "pdae_silu", "pdae_silu_bwd", "pdae_subsample2", "pdae_zero_insert2", "pdae_axpby", "pdae_embedding", "pdae_embedding_bwd", "pdae_to_nhwc",
            "pdae_from_nhwc", "pdae_softmax", "pdae_softmax_bwd", "pdae_colsum_workspace_bytes", "pdae_colsum", "pdae_linear_bwd_group", "pdae_comm_unique_id", "pdae_comm_init", "pdae_allreduce_bucket", "pdae_comm_destroy", "pdae_linear_group", "pdae_attn_fused_ok", "pdae_attn_fwd", "pdae_attn_bwd", "pdae_q_sample", "pdae_loss",
            "pdae_ddim_step", "pdae_ddpm_step", "pdae_axpby_rows", "pdae_ddim_step_rows", "pdae_ddpm_step_rows", "pdae_adam_ema", "pdae_run_ops",
-           "pdae_ssim_mse_workspace_bytes", "pdae_ssim_mse", "pdae_image_prepare_workspace_bytes", "pdae_image_prepare"]
+           "pdae_ssim_mse_workspace_bytes", "pdae_ssim_mse", "pdae_image_prepare_workspace_bytes", "pdae_image_prepare",
+           "pdae_layernorm_workspace_bytes", "pdae_layernorm_fwd", "pdae_layernorm_bwd", "pdae_dropout_fwd", "pdae_dropout_bwd", "pdae_mha_workspace_bytes",
+           "pdae_mha_fwd", "pdae_mha_bwd"]
 
 
 class SaturationGuard:
@@ -595,6 +611,74 @@ def op_softmax_bwd(p, dp, rows, T):
 
 def op_colsum(x, M, C, out, ws, acc=0):
     return make_op(OP_COLSUM, [x, out, ws], [M, C, acc])
+
+
+def _ws_bytes(ws, ws_bytes):
+    """Size of a workspace argument: given for raw pointers and plan-patched slots, else the tensor's own."""
+    if ws_bytes is not None or ws is None or isinstance(ws, int):
+        return int(ws_bytes or 0)
+    return ws.numel() * ws.element_size()
+
+
+def layernorm_ws_bytes(R, C):
+    """Workspace of the weight gradients in op_layernorm_bwd (pdae_layernorm_workspace_bytes)."""
+    return int(lib().pdae_layernorm_workspace_bytes(int(R), int(C)))
+
+
+def op_layernorm_fwd(x, gamma, beta, R, C, eps, y, mean=None, rstd=None, dtype=DT_F32, ldx=None, ldy=None):
+    """y = LayerNorm(x) over rows of C channels (pdae_layernorm_fwd).  ldx / ldy: row strides in elements (C when None)."""
+    return make_op(OP_LAYERNORM_FWD, [x, gamma, beta, y, mean, rstd], [R, C, dtype, C if ldx is None else ldx, C if ldy is None else ldy], [eps])
+
+
+def op_layernorm_bwd(x, gamma, mean, rstd, dy, R, C, dx, dgamma=None, dbeta=None, ws=None, add=None, acc_param=0, dtype=DT_F32, ldx=None, lddy=None, ldadd=None,
+                     lddx=None, ws_bytes=None):
+    """dx = LayerNorm backward (+ add), dgamma / dbeta (+)= sums over the rows (pdae_layernorm_bwd; ws: layernorm_ws_bytes)."""
+    ld = [C if v is None else v for v in (ldx, lddy, ldadd, lddx)]
+    return make_op(OP_LAYERNORM_BWD, [x, gamma, mean, rstd, dy, add, dx, dgamma, dbeta, ws], [R, C, dtype] + ld + [acc_param, _ws_bytes(ws, ws_bytes)])
+
+
+def op_dropout_fwd(x, res, n, p, y, seed=0, offset=0, layer=0, dtype=DT_F32):
+    """y = (res +) dropout(x) (pdae_dropout_fwd).  (seed, offset = step) are what Plan.set_dropout refreshes; layer: a number per call site."""
+    return make_op(OP_DROPOUT_FWD, [x, res, y], [n, dtype, seed, offset, layer], [p])
+
+
+def op_dropout_bwd(dy, n, p, dx, seed=0, offset=0, layer=0, acc=0, dtype=DT_F32):
+    """dx (+)= dy * the forward's mask / (1 - p), regenerated from the same (seed, offset, layer) (pdae_dropout_bwd)."""
+    return make_op(OP_DROPOUT_BWD, [dy, dx], [n, dtype, seed, offset, layer, acc], [p])
+
+
+class Mha:
+    """Geometry of one attention (pdae_mha_desc): q [B][Tq][Hq][D], k / v [B][Tk][Hkv][D], o like q -- or any (batch, token, head) strides in elements."""
+
+    def __init__(self, B, Tq, Tk, Hq, Hkv, D, dtype=DT_F32, causal=False, scale=None, q_stride=None, k_stride=None, v_stride=None, o_stride=None):
+        self.B, self.Tq, self.Tk, self.Hq, self.Hkv, self.D = B, Tq, Tk, Hq, Hkv, D
+        self.dtype, self.causal = dtype, bool(causal)
+        self.scale = 1.0 / D ** 0.5 if scale is None else float(scale)
+        q, k = (Tq * Hq * D, Hq * D, D), (Tk * Hkv * D, Hkv * D, D)
+        self.q_stride, self.k_stride = tuple(q_stride or q), tuple(k_stride or k)
+        self.v_stride, self.o_stride = tuple(v_stride or k), tuple(o_stride or q)
+
+    def fields(self):
+        return [self.B, self.Tq, self.Tk, self.Hq, self.Hkv, self.D, self.dtype, int(self.causal), *self.q_stride, *self.k_stride, *self.v_stride, *self.o_stride]
+
+    def cdesc(self):
+        f = [int(v) for v in self.fields()]
+        return MhaDesc(*f[:8], *((ctypes.c_int64 * 3)(*f[k:k + 3]) for k in (8, 11, 14, 17)), self.scale)
+
+    def ws_bytes(self, backward=False):
+        """Workspace of op_mha_fwd, or of one buffer that serves the forward and the backward (pdae_mha_workspace_bytes)."""
+        d = self.cdesc()
+        return int(lib().pdae_mha_workspace_bytes(ctypes.byref(d), int(backward)))
+
+
+def op_mha_fwd(a, q, k, v, o, lse=None, q_len=None, k_len=None, ws=None, ws_bytes=None):
+    """o = attention of geometry a (pdae_mha_fwd); lse [B][Hq][Tq] when a backward follows."""
+    return make_op(OP_MHA_FWD, [q, k, v, o, lse, q_len, k_len, ws], a.fields() + [_ws_bytes(ws, ws_bytes)], [a.scale])
+
+
+def op_mha_bwd(a, q, k, v, o, lse, d_o, dq, dk, dv, q_len=None, k_len=None, ws=None, ws_bytes=None):
+    """dq, dk, dv of geometry a, in the strides of q, k, v (pdae_mha_bwd)."""
+    return make_op(OP_MHA_BWD, [q, k, v, o, lse, d_o, dq, dk, dv, q_len, k_len, ws], a.fields() + [_ws_bytes(ws, ws_bytes)], [a.scale])
 
 
 def op_memset(dst, nbytes):

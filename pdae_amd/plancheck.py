@@ -28,7 +28,8 @@ _W = {
     "OP_AXPBY": (1,), "OP_EMBEDDING": (2,), "OP_EMBEDDING_BWD": (2,), "OP_TO_NHWC": (1,), "OP_FROM_NHWC": (1,), "OP_Q_SAMPLE": (5,),
     "OP_LOSS": (6, 7, 8, 9), "OP_DDIM_STEP": (3,), "OP_DDPM_STEP": (4,), "OP_AXPBY_ROWS": (4,), "OP_DDIM_STEP_ROWS": (4,),
     "OP_DDPM_STEP_ROWS": (6,), "OP_ADAM_EMA": (0, 2, 3, 4, 5), "OP_SOFTMAX": (0,), "OP_SOFTMAX_BWD": (1,), "OP_COLSUM": (1, 2), "OP_MEMSET": (0,),
-    "OP_COPY": (1,),
+    "OP_COPY": (1,), "OP_LAYERNORM_FWD": (3, 4, 5), "OP_LAYERNORM_BWD": (6, 7, 8, 9), "OP_DROPOUT_FWD": (2,), "OP_DROPOUT_BWD": (1,),
+    "OP_MHA_FWD": (3, 4, 7), "OP_MHA_BWD": (6, 7, 8, 11),
 }
 _TABLE_OPS = ("OP_LINEAR_GROUP", "OP_LINEAR_BWD_GROUP", "OP_CONV_WPREP_GROUP")      # operands in a device table: need op.rw
 WRITES = {getattr(H, k): frozenset(v) for k, v in _W.items() if hasattr(H, k)}

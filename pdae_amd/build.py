@@ -17,7 +17,10 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", 
 # no packed fp32 instructions (v_pk_add / mul / fma_f32): the compiler forms them from ordinary float code, and some of their forms have given wrong
 # results on this chip.  conv3x3y's schedule and its hazard scan are pinned with them, so the sources of that time keep their flags.
 NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-EXTRA_FLAGS = {s: NO_PACKED for s in ("layernorm.hip", "dropout.hip", "mha_fwd.hip", "mha_bwd.hip")}
+# attention: matrix instructions write vector registers (the softmax between the products reads them there; in accumulator registers every score is moved
+# twice, which was 190 of 530 instructions of the dK / dV loop)
+MFMA_VGPR = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+EXTRA_FLAGS = {"layernorm.hip": NO_PACKED, "dropout.hip": NO_PACKED, "mha_fwd.hip": NO_PACKED + MFMA_VGPR, "mha_bwd.hip": NO_PACKED + MFMA_VGPR}
 # sources whose device assembly is scanned for the store-operand hazards of isa_hazard.py after compilation: a hit FAILS the build
 HAZARD_SCAN = ["conv3x3y.hip"]
 

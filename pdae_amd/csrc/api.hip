@@ -816,6 +816,10 @@ static int mha_params(const pdae_mha_desc* d, int backward, MhaParams& P) {
   for (int j = 0; j < 3; ++j)
     for (const int64_t* st : {d->q_stride, d->k_stride, d->v_stride, d->o_stride})
       PDAE_CHECK_ARG(st[j] >= 0 && st[j] < (1ll << 40), "mha: stride %lld is out of range", (long long)st[j]);
+  // kernels address inside a tile of at most 256 rows (or one row's heads) with 31 bits from a 64-bit tile address
+  PDAE_CHECK_ARG(256 * (d->q_stride[1] > d->k_stride[1] ? d->q_stride[1] : d->k_stride[1]) < (1 << 29) && 256 * (d->v_stride[1] > d->o_stride[1] ? d->v_stride[1] : d->o_stride[1]) < (1 << 29) &&
+                     (long long)d->Hq * d->q_stride[2] < (d->Hq > 1 && d->Tq * (long long)(d->Hq / d->Hkv) <= 128 ? 1ll << 28 : 1ll << 62),
+                 "mha: a token or head stride is too long for one tile (token strides below 2^21 elements)");
   PDAE_CHECK_ARG(mha_rows_disjoint(d->o_stride, d->B, d->Tq, d->Hq, d->D), "mha: rows of o overlap (strides %lld, %lld, %lld)", (long long)d->o_stride[0],
                  (long long)d->o_stride[1], (long long)d->o_stride[2]);
   if (backward) {

@@ -107,57 +107,84 @@ __device__ __forceinline__ void mh_zero(mh_f32x16& a) {
   for (int r = 0; r < 16; ++r) a[r] = 0.f;
 }
 
-// Eight channels [c, c + 8) of one token as fp32; channels >= D read as zero and are not touched.
-template <typename T> __device__ __forceinline__ void mh_load8(const T* p, int c, int D, float (&e)[8]) {
-  if (c + 8 <= D) TkVec<T>::load8(p + c, e);
-  else {
+// ---- global loads.  Everything goes through buffer instructions: a lane whose row or channel does not exist passes an offset beyond num_records and
+// gets zeros without touching memory, so the loops have no divergent branch (those cost the kernels a wait per load).  The resource starts at the
+// tile's own first row (a 64-bit scalar address): only the distance inside a tile has to fit 31 bits, which the host checks.
+// WH (whole): D is a multiple of 8, a chunk of 8 channels is one or two 16-byte loads.  !WH: single elements, any D.
+#define MH_OOB 0xffffffffu
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mh_rsrc(const void* p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0x7fffffff, 0x00020000); }
+template <typename T, bool WH> __device__ __forceinline__ void mh_raw8(__amdgpu_buffer_rsrc_t s, unsigned off, int left, unsigned (&r)[sizeof(T) * 2]) {
+  if constexpr (WH) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = c + j < D ? TkVec<T>::load(p + c + j) : 0.f;
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
+      const tk_u32x4 v = __builtin_bit_cast(tk_u32x4, __builtin_amdgcn_raw_buffer_load_b128(s, (int)(off == MH_OOB ? MH_OOB : off + 16 * k), 0, 0));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[4 * k + j] = v[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) * 2; ++j) r[j] = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {                          // `left`: channels of this chunk that exist
+      const int o = (int)(off == MH_OOB || j >= left ? MH_OOB : off + j * (unsigned)sizeof(T));
+      if constexpr (sizeof(T) == 4) r[j] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(s, o, 0, 0);
+      else r[j / 2] |= (unsigned)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(s, o, 0, 0) << (16 * (j & 1));
+    }
   }
 }
-// B (or A) fragments of this lane's token row, straight from global memory: channels ks * 16 + h * 8 ..+7 of every k-step.  valid = 0: zeros.
-template <typename T, int NP, int DP> __device__ __forceinline__ void mh_row_frags(const T* row, bool valid, int D, int h, mh_bf16x8 (&f)[DP / 16][NP]) {
+template <typename T, int NP> __device__ __forceinline__ void mh_raw_planes(const unsigned (&r)[sizeof(T) * 2], mh_bf16x8 (&f)[NP]) {
+  if constexpr (NP == 1) { const tk_u32x4 v = {r[0], r[1], r[2], r[3]}; f[0] = __builtin_bit_cast(mh_bf16x8, v); }
+  else {
+    float e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = __uint_as_float(r[j % (sizeof(T) * 2)]);
+    mh_planes<NP>(e, f);
+  }
+}
+// B fragments of this lane's token row, straight from global memory: channels ks * 16 + h * 8 ..+7 of every k-step.  off: the row's byte offset from
+// `base` (MH_OOB: the row does not exist, zeros).
+template <typename T, int NP, int DP, bool WH> __device__ __forceinline__ void mh_row_frags(const T* base, unsigned off, int D, int h, mh_bf16x8 (&f)[DP / 16][NP]) {
+  const __amdgpu_buffer_rsrc_t s = mh_rsrc(base);
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) {
-    float e[8];
-    if (valid) mh_load8(row, ks * 16 + h * 8, D, e);
-    else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = 0.f;
-    }
-    mh_planes<NP>(e, f[ks]);
+    const int c = ks * 16 + h * 8;
+    unsigned r[sizeof(T) * 2];
+    mh_raw8<T, WH>(s, off == MH_OOB || c >= D ? MH_OOB : off + c * (unsigned)sizeof(T), D - c, r);
+    mh_raw_planes<T, NP>(r, f[ks]);
   }
 }
 
-// ---- token-major LDS tile [plane][ROWS][DP + 8] bf16: rows 16 bytes off a multiple of 128 keep ds_read_b128 of 32 rows at one channel free of conflicts
-#define MH_PAD 8
+// ---- token-major LDS tile [plane][ROWS][LD] bf16 in 16-byte chunks, chunk c of row r at position c ^ mh_swz(r).  64 banks of 4 bytes: a row read (16 lanes =
+// 16 consecutive rows, one chunk each) and a transposing read (32 lanes = 4 rows x 4 chunks) both touch every bank once.  With rows padded by 16 bytes
+// instead, the four rows of a transposing read overlapped in up to four ways: half of all LDS cycles of the kernels were conflicts.
+template <int DP> struct MhLd { static constexpr int NC = DP <= 32 ? 4 : DP <= 64 ? 8 : 16, LD = NC * 8; };      // chunks of a row (a power of two), elements
+template <int DP> __device__ __forceinline__ int mh_swz(int row) {
+  constexpr int NC = MhLd<DP>::NC, RPL = 16 / NC, NB = NC / 4;          // rows that share a 256-byte line; 64-byte blocks of a row
+  return ((row / RPL) % NB) * 4 + ((row / RPL / NB) & 3);
+}
 template <int NP, int ROWS, int DP> struct MhTile {
-  static constexpr int LD = DP + MH_PAD, PLANE = ROWS * LD, ELEMS = NP * PLANE;
+  static constexpr int LD = MhLd<DP>::LD, PLANE = ROWS * LD, ELEMS = NP * PLANE;
 };
 // Global -> registers -> LDS of ROWS tokens by 256 threads: chunks of 8 channels.
-template <typename T, int NP, int ROWS, int DP> struct MhStage {
-  static constexpr int CPR = DP / 8, CH = ROWS * CPR, N = (CH + 255) / 256, LD = DP + MH_PAD, PLANE = ROWS * LD;
-  static constexpr int W = sizeof(T) == 2 ? 4 : 8;         // dwords a chunk holds in registers
-  unsigned r[N][W];
-  // tokens [row0, row0 + ROWS) of base (token stride `st` elements); those outside [lo, hi) and channels >= D come as zero and are never read
-  __device__ __forceinline__ void load(const T* base, long long st, int row0, int lo, int hi, int D) {
+template <typename T, int NP, int ROWS, int DP, bool WH> struct MhStage {
+  static constexpr int CPR = DP / 8, CH = ROWS * CPR, N = (CH + 255) / 256, LD = MhLd<DP>::LD, PLANE = ROWS * LD, W = sizeof(T) * 2;
+  unsigned r[N][W], off[N];                                // chunk in flight; its byte offset from the tile's first row
+  int D;
+  __device__ __forceinline__ void init(long long stride, int D_) {
+    D = D_;
 #pragma unroll
     for (int l = 0; l < N; ++l) {
-      const int i = threadIdx.x + 256 * l, row = row0 + i / CPR, c = (i % CPR) * 8;
+      const int i = threadIdx.x + 256 * l, c = (i % CPR) * 8;
+      off[l] = (CH % 256 == 0 || i < CH) && c < D ? (unsigned)((i / CPR) * stride + c) * (unsigned)sizeof(T) : MH_OOB;
+    }
+  }
+  // tokens [row0, row0 + ROWS) of base (token stride `stride` elements); those outside [lo, hi) come as zero and are never read
+  __device__ __forceinline__ void load(const T* base, long long stride, int row0, int lo, int hi) {
+    const __amdgpu_buffer_rsrc_t s = mh_rsrc(base + (long long)row0 * stride);
 #pragma unroll
-      for (int j = 0; j < W; ++j) r[l][j] = 0;
-      if ((CH % 256 == 0 || i < CH) && row >= lo && row < hi && c < D) {
-        const T* p = base + (long long)row * st + c;
-        if (c + 8 <= D) __builtin_memcpy(r[l], p, 8 * sizeof(T));
-        else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (c + j < D) {
-              if constexpr (sizeof(T) == 4) r[l][j] = __float_as_uint(TkVec<T>::load(p + j));
-              else r[l][j / 2] |= (unsigned)__builtin_bit_cast(unsigned short, p[j]) << (16 * (j & 1));
-            }
-        }
-      }
+    for (int l = 0; l < N; ++l) {
+      const int i = threadIdx.x + 256 * l, row = row0 + i / CPR;
+      mh_raw8<T, WH>(s, row >= lo && row < hi ? off[l] : MH_OOB, D - (i % CPR) * 8, r[l]);
     }
   }
   __device__ __forceinline__ void store(unsigned short* lds) const {
@@ -165,45 +192,40 @@ template <typename T, int NP, int ROWS, int DP> struct MhStage {
     for (int l = 0; l < N; ++l) {
       const int i = threadIdx.x + 256 * l;
       if (CH % 256 != 0 && i >= CH) continue;
-      unsigned short* d = lds + (i / CPR) * LD + (i % CPR) * 8;
-      if constexpr (NP == 1) *reinterpret_cast<tk_u32x4*>(d) = tk_u32x4{r[l][0], r[l][1], r[l][2], r[l][3]};
-      else {
-        float e[8];
+      unsigned short* d = lds + (i / CPR) * LD + ((i % CPR) ^ mh_swz<DP>(i / CPR)) * 8;
+      mh_bf16x8 f[NP];
+      mh_raw_planes<T, NP>(r[l], f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = __uint_as_float(r[l][j % W]);
-        mh_bf16x8 f[NP];
-        mh_planes<NP>(e, f);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) *reinterpret_cast<mh_bf16x8*>(d + p * PLANE) = f[p];
-      }
+      for (int p = 0; p < NP; ++p) *reinterpret_cast<mh_bf16x8*>(d + p * PLANE) = f[p];
     }
   }
 };
-// A fragment, tokens on rows: token row0 + l%32, channels ks * 16 + h * 8 ..+7
+// A fragment, tokens on rows: token row0 + l%32 (row0 a multiple of 32), channels ks * 16 + h * 8 ..+7
 template <int NP, int ROWS, int DP> __device__ __forceinline__ void mh_frag_rows(const unsigned short* lds, int row0, int ks, int li, int h, mh_bf16x8 (&f)[NP]) {
+  constexpr int LD = MhLd<DP>::LD;
 #pragma unroll
   for (int p = 0; p < NP; ++p)
-    f[p] = *reinterpret_cast<const mh_bf16x8*>(lds + p * MhTile<NP, ROWS, DP>::PLANE + (row0 + li) * MhTile<NP, ROWS, DP>::LD + ks * 16 + h * 8);
+    f[p] = *reinterpret_cast<const mh_bf16x8*>(lds + p * MhTile<NP, ROWS, DP>::PLANE + row0 * LD + li * LD + ((ks * 2 + h) ^ mh_swz<DP>(li)) * 8);
 }
-// A fragment, channels db * 32 + l%32 on rows, k = the sixteen tokens from row0 in the order of packed accumulator registers
+// A fragment, channels db * 32 + l%32 on rows, k = the sixteen tokens from row0 (a multiple of 16) in the order of packed accumulator registers
 template <int NP, int ROWS, int DP> __device__ __forceinline__ void mh_frag_cols(const unsigned short* lds, int row0, int db, int lane, mh_bf16x8 (&f)[NP]) {
-  constexpr int LD = MhTile<NP, ROWS, DP>::LD;
-  const int i = lane & 15, g = (lane >> 4) & 1, h = lane >> 5;
+  constexpr int LD = MhLd<DP>::LD;
+  const int i = lane & 15, g = (lane >> 4) & 1, h = lane >> 5, r = 4 * h + (i >> 2), c = db * 4 + g * 2 + ((i & 3) >> 1);
 #pragma unroll
   for (int p = 0; p < NP; ++p) {
-    const unsigned short* a = lds + p * MhTile<NP, ROWS, DP>::PLANE + (row0 + 4 * h + (i >> 2)) * LD + db * 32 + g * 16 + (i & 3) * 4;
-    const mh_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mh_lds4)(a));
-    const mh_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mh_lds4)(a + 8 * LD));
+    const unsigned short* a = lds + p * MhTile<NP, ROWS, DP>::PLANE + row0 * LD + (i & 1) * 4;
+    const mh_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mh_lds4)(a + r * LD + (c ^ mh_swz<DP>(r)) * 8));
+    const mh_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mh_lds4)(a + (r + 8) * LD + (c ^ mh_swz<DP>(r + 8)) * 8));
     const mh_s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     f[p] = __builtin_bit_cast(mh_bf16x8, v);
   }
 }
 // Stores the four channels [c, c + 4) of one token row.
-template <typename T> __device__ __forceinline__ void mh_store4(T* row, int c, int D, float a, float b, float e, float d) {
-  if (c + 4 <= D) {
+template <typename T, bool WH> __device__ __forceinline__ void mh_store4(T* row, int c, int D, float a, float b, float e, float d) {
+  if (WH ? c < D : c + 4 <= D) {
     if constexpr (sizeof(T) == 2) { const unsigned w[2] = {tk_pack2(a, b), tk_pack2(e, d)}; __builtin_memcpy(row + c, w, 8); }
     else { const float w[4] = {a, b, e, d}; __builtin_memcpy(row + c, w, 16); }
-  } else {
+  } else if constexpr (!WH) {
     if (c < D) TkVec<T>::store(row + c, a);
     if (c + 1 < D) TkVec<T>::store(row + c + 1, b);
     if (c + 2 < D) TkVec<T>::store(row + c + 2, e);

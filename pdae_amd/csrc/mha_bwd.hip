@@ -23,8 +23,14 @@ template <typename T> __global__ void __launch_bounds__(256) mha_delta_kernel(co
   if (tq < lq && c < P.D) {
     float x[8], y[8];
     const long long at = b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh;
-    mh_load8((const T*)P.o + at, c, P.D, x);
-    mh_load8((const T*)P.d_o + at, c, P.D, y);
+    if (c + 8 <= P.D) { TkVec<T>::load8((const T*)P.o + at + c, x); TkVec<T>::load8((const T*)P.d_o + at + c, y); }
+    else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = c + j < P.D ? TkVec<T>::load((const T*)P.o + at + c + j) : 0.f;
+        y[j] = c + j < P.D ? TkVec<T>::load((const T*)P.d_o + at + c + j) : 0.f;
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) s += x[j] * y[j];
   }
@@ -34,17 +40,17 @@ template <typename T> __global__ void __launch_bounds__(256) mha_delta_kernel(co
 }
 
 // accumulators (channels on rows, this lane's token on the column) -> row of a tensor, or fp32 partial row
-template <typename T, int DB> __device__ __forceinline__ void mh_put(const mh_f32x16 (&a)[DB], float f, bool keep, T* row, int D, int h) {
+template <typename T, int DB, bool WH> __device__ __forceinline__ void mh_put(const mh_f32x16 (&a)[DB], float f, bool keep, T* row, int D, int h) {
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int c = d * 32 + g * 8 + h * 4;
-      mh_store4<T>(row, c, D, keep ? a[d][g * 4] * f : 0.f, keep ? a[d][g * 4 + 1] * f : 0.f, keep ? a[d][g * 4 + 2] * f : 0.f, keep ? a[d][g * 4 + 3] * f : 0.f);
+      mh_store4<T, WH>(row, c, D, keep ? a[d][g * 4] * f : 0.f, keep ? a[d][g * 4 + 1] * f : 0.f, keep ? a[d][g * 4 + 2] * f : 0.f, keep ? a[d][g * 4 + 3] * f : 0.f);
     }
 }
 
-template <typename T, int DP, int KT, int OCC>
+template <typename T, int DP, int KT, int OCC, bool WH>
 __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
   constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, KB = KT / 32;
   constexpr int TE = MhTile<NP, KT, DP>::ELEMS;
@@ -67,8 +73,10 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
   const bool wlive = __any(ok);
 
   mh_bf16x8 Q[KS][NP], G[KS][NP];
-  mh_row_frags<T, NP, DP>((const T*)P.q + b * P.qb + (long long)tq * P.qt + (long long)hq * P.qh, ok, P.D, h, Q);
-  mh_row_frags<T, NP, DP>((const T*)P.d_o + b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh, ok, P.D, h, G);
+  mh_row_frags<T, NP, DP, WH>((const T*)P.q + b * P.qb + (long long)row0 * P.qt + (long long)hq * P.qh,
+                              ok ? (unsigned)((tq - row0) * P.qt) * (unsigned)sizeof(T) : MH_OOB, P.D, h, Q);
+  mh_row_frags<T, NP, DP, WH>((const T*)P.d_o + b * P.ob + (long long)row0 * P.ot + (long long)hq * P.oh,
+                              ok ? (unsigned)((tq - row0) * P.ot) * (unsigned)sizeof(T) : MH_OOB, P.D, h, G);
   float lse2 = MH_INF, del = 0.f;
   if (ok) {
     const long long i = ((long long)b * P.Hq + hq) * P.Tq + tq;
@@ -80,10 +88,11 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
 #pragma unroll
   for (int d = 0; d < DB; ++d) mh_zero(dQ[d]);
 
-  MhStage<T, NP, KT, DP> sk, sv;
+  MhStage<T, NP, KT, DP, WH> sk, sv;
+  sk.init(P.kt, P.D); sv.init(P.vt, P.D);
   if (tb < te) {
-    sk.load(kbase, P.kt, tb * KT, 0, lk, P.D);
-    sv.load(vbase, P.vt, tb * KT, 0, lk, P.D);
+    sk.load(kbase, P.kt, tb * KT, 0, lk);
+    sv.load(vbase, P.vt, tb * KT, 0, lk);
     sk.store(mh_sm); sv.store(mh_sm + TE);
   }
   __syncthreads();
@@ -91,7 +100,7 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
     const unsigned short* cur = mh_sm + ((it - tb) & 1) * 2 * TE;
     unsigned short* nxt = mh_sm + (((it - tb) & 1) ^ 1) * 2 * TE;
     const bool more = it + 1 < te;
-    if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk, P.D); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk, P.D); }
+    if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk); }
     const int k0 = it * KT;
     if (wlive && __any(kmax > k0)) {
 #pragma unroll
@@ -137,13 +146,13 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
   if (tq >= P.Tq) return;
   if (P.splits > 1) {
     float* row = P.part + (((long long)split * P.B * P.Hq + unit) * P.Tq + tq) * P.D;
-    mh_put<float, DB>(dQ, P.scale, ok, row, P.D, h);
+    mh_put<float, DB, WH>(dQ, P.scale, ok, row, P.D, h);
   } else {
-    mh_put<T, DB>(dQ, P.scale, ok, (T*)P.dq + b * P.qb + (long long)tq * P.qt + (long long)hq * P.qh, P.D, h);
+    mh_put<T, DB, WH>(dQ, P.scale, ok, (T*)P.dq + b * P.qb + (long long)tq * P.qt + (long long)hq * P.qh, P.D, h);
   }
 }
 
-template <typename T, int DP, int QT, int OCC>
+template <typename T, int DP, int QT, int OCC, bool WH, bool KL>
 __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
   constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, QB = QT / 32;
   constexpr int TE = MhTile<NP, QT, DP>::ELEMS, BUF = 2 * TE + 4 * QT;         // Q tile | dO tile | lse2[QT], delta[QT] (floats)
@@ -158,58 +167,76 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
   const int qlo = P.causal ? max(0, -off) : 0;                                 // first query that sees a key
   const int first = P.causal ? max(qlo, key0 - off) : 0;                       // first query that sees key0
   const int q0t = first / QT, nq = key0 < lk && first < lq ? (lq + QT - 1) / QT - q0t : 0;
-  const long long items = (long long)nq * P.G;
-  const long long ib = items * split / P.splits, ie = items * (split + 1) / P.splits;
+  const int items = nq * P.G;                                                  // (query head, query tile) pairs in order (the host checks G * tiles < 2^31)
+  const int ib = (int)((long long)items * split / P.splits), ie = (int)((long long)items * (split + 1) / P.splits);
+  int lh = nq > 0 ? ib / nq : 0, lt = nq > 0 ? ib - lh * nq : 0;               // the pair that is loaded next
 
   mh_bf16x8 K[KS][NP], V[KS][NP];
-  mh_row_frags<T, NP, DP>((const T*)P.k + b * P.kb + (long long)key * P.kt + (long long)hk * P.kh, ok, P.D, h, K);
-  mh_row_frags<T, NP, DP>((const T*)P.v + b * P.vb + (long long)key * P.vt + (long long)hk * P.vh, ok, P.D, h, V);
+  mh_row_frags<T, NP, DP, WH>((const T*)P.k + b * P.kb + (long long)key0 * P.kt + (long long)hk * P.kh,
+                              ok ? (unsigned)((key - key0) * P.kt) * (unsigned)sizeof(T) : MH_OOB, P.D, h, K);
+  mh_row_frags<T, NP, DP, WH>((const T*)P.v + b * P.vb + (long long)key0 * P.vt + (long long)hk * P.vh,
+                              ok ? (unsigned)((key - key0) * P.vt) * (unsigned)sizeof(T) : MH_OOB, P.D, h, V);
+  // KL: this wave's K fragments live in LDS (a lane reads back its own 16 bytes) instead of 4 KS NP registers
+  unsigned short* kl = mh_sm + 2 * BUF + wv * (KS * NP * 512) + lane * 8;
+  if constexpr (KL) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) *reinterpret_cast<mh_bf16x8*>(kl + (ks * NP + p) * 512) = K[ks][p];
+  }
   mh_f32x16 dK[DB], dV[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) { mh_zero(dK[d]); mh_zero(dV[d]); }
 
-  MhStage<T, NP, QT, DP> sq, sg;
+  MhStage<T, NP, QT, DP, WH> sq, sg;
+  sq.init(P.qt, P.D); sg.init(P.ot, P.D);
   float rl = 0.f, rd = 0.f;
-  auto load = [&](long long it) {
-    const int hq = hk * P.G + (int)(it / nq), q0 = (q0t + (int)(it % nq)) * QT;
-    sq.load((const T*)P.q + b * P.qb + (long long)hq * P.qh, P.qt, q0, qlo, lq, P.D);
-    sg.load((const T*)P.d_o + b * P.ob + (long long)hq * P.oh, P.ot, q0, qlo, lq, P.D);
-    if (t < QT) {
-      const int tq = q0 + t;
-      rl = MH_INF; rd = 0.f;
-      if (tq >= qlo && tq < lq) {
-        const long long i = ((long long)b * P.Hq + hq) * P.Tq + tq;
-        const float e = P.lse[i];
-        rl = e == -MH_INF ? MH_INF : e * MH_LOG2E;
-        rd = P.delta[i];
-      }
-    }
+  auto load = [&]() {
+    const int hq = hk * P.G + lh, q0 = (q0t + lt) * QT;
+    sq.load((const T*)P.q + b * P.qb + (long long)hq * P.qh, P.qt, q0, qlo, lq);
+    sg.load((const T*)P.d_o + b * P.ob + (long long)hq * P.oh, P.ot, q0, qlo, lq);
+    // rows that do not count come as lse = +inf: their probabilities are exact zeros
+    const int tq = q0 + (t & (QT - 1));
+    const bool in = tq >= qlo && tq < lq;
+    const long long i = ((long long)b * P.Hq + hq) * P.Tq + (in ? tq : 0);
+    const float e = P.lse[i], d = P.delta[i];
+    rl = !in || e == -MH_INF ? MH_INF : e * MH_LOG2E;
+    rd = in ? d : 0.f;
+    if (++lt == nq) { lt = 0; ++lh; }
   };
   auto store = [&](unsigned short* buf) {
     sq.store(buf); sg.store(buf + TE);
     float* st = reinterpret_cast<float*>(buf + 2 * TE);
     if (t < QT) { st[t] = rl; st[QT + t] = rd; }
   };
-  if (ib < ie) { load(ib); store(mh_sm); }
+  int ct = lt;                                                                 // query tile of the pair being multiplied
+  if (ib < ie) { load(); store(mh_sm); }
   __syncthreads();
-  for (long long it = ib; it < ie; ++it) {
+  for (int it = ib; it < ie; ++it) {
     const unsigned short* cur = mh_sm + ((it - ib) & 1) * BUF;
     unsigned short* nxt = mh_sm + (((it - ib) & 1) ^ 1) * BUF;
     const bool more = it + 1 < ie;
-    if (more) load(it + 1);
-    const int q0 = (q0t + (int)(it % nq)) * QT;
+    if (more) load();
+    const int q0 = (q0t + ct) * QT;
+    if (++ct == nq) ct = 0;
     const float* st = reinterpret_cast<const float*>(cur + 2 * TE);
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       const int qa = q0 + qb * 32;
-      if (kw >= lk || (P.causal && qa + 31 + off < kw)) continue;              // no pair of this wave (uniform)
       mh_f32x16 S, E;
       mh_zero(S); mh_zero(E);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         mh_bf16x8 A[NP];
         mh_frag_rows<NP, QT, DP>(cur, qb * 32, ks, li, h, A);
-        mh_mma<NP>(A, K[ks], S);
+        if constexpr (KL) {
+          mh_bf16x8 Kf[NP];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) Kf[p] = *reinterpret_cast<const mh_bf16x8*>(kl + (ks * NP + p) * 512);
+          mh_mma<NP>(A, Kf, S);
+        } else {
+          mh_mma<NP>(A, K[ks], S);
+        }
         mh_frag_rows<NP, QT, DP>(cur + TE, qb * 32, ks, li, h, A);
         mh_mma<NP>(A, V[ks], E);
       }
@@ -227,7 +254,10 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
             const int r = s * 8 + g * 4 + j;
             float x = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], P.sc2, -l4[j]));
             float y = x * (E[r] - d4[j]);
-            if (cut && qa + 8 * (2 * s + g) + 4 * h + j + off < key) { x = 0.f; y = 0.f; }
+            if (cut) {
+              const bool see = qa + 8 * (2 * s + g) + 4 * h + j + off >= key;
+              x = see ? x : 0.f; y = see ? y : 0.f;
+            }
             p[g * 4 + j] = x; e[g * 4 + j] = y;
           }
         }
@@ -252,11 +282,11 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
   if (P.splits > 1) {
     const long long n = (long long)P.B * P.Hkv * P.Tk;
     float* row = P.part + ((long long)split * 2 * n + (long long)unit * P.Tk + key) * P.D;
-    mh_put<float, DB>(dK, P.scale, ok, row, P.D, h);
-    mh_put<float, DB>(dV, 1.f, ok, row + n * P.D, P.D, h);
+    mh_put<float, DB, WH>(dK, P.scale, ok, row, P.D, h);
+    mh_put<float, DB, WH>(dV, 1.f, ok, row + n * P.D, P.D, h);
   } else {
-    mh_put<T, DB>(dK, P.scale, ok, (T*)P.dk + b * P.kb + (long long)key * P.kt + (long long)hk * P.kh, P.D, h);
-    mh_put<T, DB>(dV, 1.f, ok, (T*)P.dv + b * P.vb + (long long)key * P.vt + (long long)hk * P.vh, P.D, h);
+    mh_put<T, DB, WH>(dK, P.scale, ok, (T*)P.dk + b * P.kb + (long long)key * P.kt + (long long)hk * P.kh, P.D, h);
+    mh_put<T, DB, WH>(dV, 1.f, ok, (T*)P.dv + b * P.vb + (long long)key * P.vt + (long long)hk * P.vh, P.D, h);
   }
 }
 
@@ -303,17 +333,17 @@ size_t k_mha_bwd_workspace_bytes(const MhaParams& P) {
   return (L.delta_floats + (L.dq_floats > L.dkv_floats ? L.dq_floats : L.dkv_floats)) * sizeof(float);
 }
 
-template <typename T, int DP, int KT, int OCC> static void mh_dq_go(const MhaParams& P, hipStream_t st) {
+template <typename T, int DP, int KT, int OCC, bool WH = true> static void mh_dq_go(const MhaParams& P, hipStream_t st) {
   constexpr int lds = 4 * MhTile<MhNP<T>::NP, KT, DP>::ELEMS * 2;
   static_assert(lds <= 163840, "LDS");
-  hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_dq_kernel<T, DP, KT, OCC>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  hipLaunchKernelGGL((mha_dq_kernel<T, DP, KT, OCC>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
+  hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_dq_kernel<T, DP, KT, OCC, WH>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL((mha_dq_kernel<T, DP, KT, OCC, WH>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
 }
-template <typename T, int DP, int QT, int OCC> static void mh_dkv_go(const MhaParams& P, hipStream_t st) {
-  constexpr int lds = 2 * (2 * MhTile<MhNP<T>::NP, QT, DP>::ELEMS + 4 * QT) * 2;
+template <typename T, int DP, int QT, int OCC, bool WH = true, bool KL = false> static void mh_dkv_go(const MhaParams& P, hipStream_t st) {
+  constexpr int lds = (2 * (2 * MhTile<MhNP<T>::NP, QT, DP>::ELEMS + 4 * QT) + (KL ? 4 * DP / 16 * MhNP<T>::NP * 512 : 0)) * 2;
   static_assert(lds <= 163840, "LDS");
-  hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_dkv_kernel<T, DP, QT, OCC>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  hipLaunchKernelGGL((mha_dkv_kernel<T, DP, QT, OCC>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
+  hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_dkv_kernel<T, DP, QT, OCC, WH, KL>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL((mha_dkv_kernel<T, DP, QT, OCC, WH, KL>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
 }
 template <typename T> static void mh_bwd_join(const float* part, long long step, int splits, void* out, long long sb, long long stt, long long sh, int H, int Tn, int D,
                                               long long rows, hipStream_t st) {
@@ -338,12 +368,14 @@ int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
     P.units = P.B * P.Hq; P.tiles = L.dq_tiles; P.splits = L.dq_splits;
     PDAE_CHECK_ARG(mh_grid(P) < (1ll << 31), "mha_bwd: too many query tiles for one launch");
     if (bf) {
-      if (P.D <= 32) mh_dq_go<tk_bf16, 32, 64, 2>(P, st);
+      if (P.D & 7) mh_dq_go<tk_bf16, 128, 64, 1, false>(P, st);
+      else if (P.D <= 32) mh_dq_go<tk_bf16, 32, 64, 2>(P, st);
       else if (P.D <= 64) mh_dq_go<tk_bf16, 64, 64, 2>(P, st);
       else if (P.D <= 96) mh_dq_go<tk_bf16, 96, 64, 2>(P, st);
-      else mh_dq_go<tk_bf16, 128, 64, 1>(P, st);
+      else mh_dq_go<tk_bf16, 128, 64, 2>(P, st);
     } else {
-      if (P.D <= 32) mh_dq_go<float, 32, 32, 2>(P, st);
+      if (P.D & 7) mh_dq_go<float, 128, 32, 1, false>(P, st);
+      else if (P.D <= 32) mh_dq_go<float, 32, 32, 2>(P, st);
       else if (P.D <= 64) mh_dq_go<float, 64, 32, 2>(P, st);
       else if (P.D <= 96) mh_dq_go<float, 96, 32, 1>(P, st);
       else mh_dq_go<float, 128, 32, 1>(P, st);
@@ -356,14 +388,16 @@ int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   }
   if (P.Tk > 0) {
     P.units = P.B * P.Hkv; P.tiles = L.dkv_tiles; P.splits = L.dkv_splits;
-    PDAE_CHECK_ARG(mh_grid(P) < (1ll << 31), "mha_bwd: too many key tiles for one launch");
+    PDAE_CHECK_ARG(mh_grid(P) < (1ll << 31) && (long long)cdiv(P.Tq, 32) * P.G < (1ll << 31), "mha_bwd: too many tiles for one launch");
     if (bf) {
-      if (P.D <= 32) mh_dkv_go<tk_bf16, 32, 32, 2>(P, st);
+      if (P.D & 7) mh_dkv_go<tk_bf16, 128, 32, 1, false>(P, st);
+      else if (P.D <= 32) mh_dkv_go<tk_bf16, 32, 32, 2>(P, st);
       else if (P.D <= 64) mh_dkv_go<tk_bf16, 64, 32, 2>(P, st);
-      else if (P.D <= 96) mh_dkv_go<tk_bf16, 96, 32, 1>(P, st);
-      else mh_dkv_go<tk_bf16, 128, 32, 1>(P, st);
+      else if (P.D <= 96) mh_dkv_go<tk_bf16, 96, 32, 2>(P, st);
+      else mh_dkv_go<tk_bf16, 128, 32, 2, true, true>(P, st);
     } else {
-      if (P.D <= 32) mh_dkv_go<float, 32, 32, 2>(P, st);
+      if (P.D & 7) mh_dkv_go<float, 128, 32, 1, false>(P, st);
+      else if (P.D <= 32) mh_dkv_go<float, 32, 32, 2>(P, st);
       else if (P.D <= 64) mh_dkv_go<float, 64, 32, 1>(P, st);
       else if (P.D <= 96) mh_dkv_go<float, 96, 32, 1>(P, st);
       else mh_dkv_go<float, 128, 32, 1>(P, st);

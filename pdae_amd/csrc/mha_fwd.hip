@@ -10,7 +10,7 @@
 #include "kernels.h"
 #include "mha.h"
 
-template <typename T, int DP, int QB, int KT, int OCC>
+template <typename T, int DP, int QB, int KT, int OCC, bool WH>
 __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
   constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, KB = KT / 32;
   constexpr int TE = MhTile<NP, KT, DP>::ELEMS;
@@ -44,7 +44,9 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
     const bool ok = r < P.R && tq < lq;
     kmax[a] = ok ? (P.causal ? min(lk, tq + off + 1) : lk) : lk;               // rows that do not exist never force the masked path; they are zeroed at the end
     live = live || ok;
-    mh_row_frags<T, NP, DP>((const T*)P.q + b * P.qb + (long long)tq * P.qt + (long long)hq * P.qh, ok, P.D, h, Q[a]);
+    const int t0 = row0 / P.GP;                                                // (the tile's first token: offsets inside a tile fit 32 bits)
+    mh_row_frags<T, NP, DP, WH>((const T*)P.q + b * P.qb + (long long)t0 * P.qt + (long long)hp * P.GP * P.qh,
+                                ok ? (unsigned)((tq - t0) * P.qt + (r % P.GP) * P.qh) * (unsigned)sizeof(T) : MH_OOB, P.D, h, Q[a]);
   }
   const bool wlive = __any(live);
   int kwave = 0;                                                               // last key any of the wave's rows sees
@@ -60,10 +62,11 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
     for (int d = 0; d < DB; ++d) mh_zero(O[a][d]);
   }
 
-  MhStage<T, NP, KT, DP> sk, sv;
+  MhStage<T, NP, KT, DP, WH> sk, sv;
+  sk.init(P.kt, P.D); sv.init(P.vt, P.D);
   if (tb < te) {
-    sk.load(kbase, P.kt, tb * KT, 0, lk, P.D);
-    sv.load(vbase, P.vt, tb * KT, 0, lk, P.D);
+    sk.load(kbase, P.kt, tb * KT, 0, lk);
+    sv.load(vbase, P.vt, tb * KT, 0, lk);
     sk.store(mh_sm); sv.store(mh_sm + TE);
   }
   __syncthreads();
@@ -71,7 +74,7 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
     const unsigned short* cur = mh_sm + ((it - tb) & 1) * 2 * TE;
     unsigned short* nxt = mh_sm + (((it - tb) & 1) ^ 1) * 2 * TE;
     const bool more = it + 1 < te;
-    if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk, P.D); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk, P.D); }
+    if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk); }
     const int k0 = it * KT;
     if (wlive && __any(kwave > k0)) {
       mh_f32x16 S[QB][KB];
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-          for (int g = 0; g < 4; ++g) mh_store4<float>(po, d * 32 + g * 8 + h * 4, P.D, O[a][d][g * 4], O[a][d][g * 4 + 1], O[a][d][g * 4 + 2], O[a][d][g * 4 + 3]);
+          for (int g = 0; g < 4; ++g) mh_store4<float, WH>(po, d * 32 + g * 8 + h * 4, P.D, O[a][d][g * 4], O[a][d][g * 4 + 1], O[a][d][g * 4 + 2], O[a][d][g * 4 + 3]);
       }
       continue;
     }
@@ -166,7 +169,7 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
       for (int g = 0; g < 4; ++g) {
         const float x0 = any ? O[a][d][g * 4] * inv : 0.f, x1 = any ? O[a][d][g * 4 + 1] * inv : 0.f;
         const float x2 = any ? O[a][d][g * 4 + 2] * inv : 0.f, x3 = any ? O[a][d][g * 4 + 3] * inv : 0.f;
-        mh_store4<T>(orow, d * 32 + g * 8 + h * 4, P.D, x0, x1, x2, x3);
+        mh_store4<T, WH>(orow, d * 32 + g * 8 + h * 4, P.D, x0, x1, x2, x3);
       }
     if (P.lse && h == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = any ? (m[a] + __builtin_amdgcn_logf(ls)) * MH_LN2 : -MH_INF;      // (v_log_f32: log2)
   }
@@ -202,7 +205,7 @@ __global__ void __launch_bounds__(256) mha_join_kernel(const MhaParams P) {
 }
 
 // ---- host: row packing, key ranges
-static int mh_qb(int dtype, int R, int D) { return dtype == PDAE_DT_BF16 && R > 128 && D <= 64 ? 2 : 1; }
+static int mh_qb(int dtype, int R, int D) { return dtype == PDAE_DT_BF16 && R > 128 && D <= 64 && D % 8 == 0 ? 2 : 1; }
 // Rows of a tile: with few query tokens the G heads that share a key head become rows of one tile, so its keys are read once for all of them.
 // Then, when the tiles alone do not give every CU two workgroups, the keys are split into ranges of at least 256.
 static void mh_fwd_plan(MhaParams& P, int dtype) {
@@ -226,12 +229,12 @@ size_t k_mha_fwd_workspace_bytes(const MhaParams& P0, int dtype) {
   return mh_fwd_part_floats(P) * sizeof(float);
 }
 
-template <typename T, int DP, int QB, int KT, int OCC> static void mh_fwd_go(const MhaParams& P, hipStream_t st) {
+template <typename T, int DP, int QB, int KT, int OCC, bool WH = true> static void mh_fwd_go(const MhaParams& P, hipStream_t st) {
   constexpr int NP = MhNP<T>::NP;
   const size_t lds = (size_t)4 * MhTile<NP, KT, DP>::ELEMS * 2;
   static_assert(4 * MhTile<NP, KT, DP>::ELEMS * 2 <= 163840, "LDS");
-  hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_fwd_kernel<T, DP, QB, KT, OCC>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  hipLaunchKernelGGL((mha_fwd_kernel<T, DP, QB, KT, OCC>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
+  hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_fwd_kernel<T, DP, QB, KT, OCC, WH>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  hipLaunchKernelGGL((mha_fwd_kernel<T, DP, QB, KT, OCC, WH>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
 }
 
 int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStream_t st) {
@@ -244,12 +247,14 @@ int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   P.part = (float*)ws;
   const int qb = mh_qb(dtype, P.R, P.D);
   if (dtype == PDAE_DT_BF16) {
-    if (P.D <= 32) { if (qb == 2) mh_fwd_go<tk_bf16, 32, 2, 64, 2>(P, st); else mh_fwd_go<tk_bf16, 32, 1, 64, 2>(P, st); }
+    if (P.D & 7) mh_fwd_go<tk_bf16, 128, 1, 64, 2, false>(P, st);
+    else if (P.D <= 32) { if (qb == 2) mh_fwd_go<tk_bf16, 32, 2, 64, 2>(P, st); else mh_fwd_go<tk_bf16, 32, 1, 64, 2>(P, st); }
     else if (P.D <= 64) { if (qb == 2) mh_fwd_go<tk_bf16, 64, 2, 64, 2>(P, st); else mh_fwd_go<tk_bf16, 64, 1, 64, 2>(P, st); }
     else if (P.D <= 96) mh_fwd_go<tk_bf16, 96, 1, 64, 2>(P, st);
     else mh_fwd_go<tk_bf16, 128, 1, 64, 2>(P, st);
   } else {
-    if (P.D <= 32) mh_fwd_go<float, 32, 1, 32, 2>(P, st);
+    if (P.D & 7) mh_fwd_go<float, 128, 1, 32, 1, false>(P, st);
+    else if (P.D <= 32) mh_fwd_go<float, 32, 1, 32, 2>(P, st);
     else if (P.D <= 64) mh_fwd_go<float, 64, 1, 32, 2>(P, st);
     else if (P.D <= 96) mh_fwd_go<float, 96, 1, 32, 1>(P, st);
     else mh_fwd_go<float, 128, 1, 32, 1>(P, st);

@@ -24,6 +24,8 @@ typedef __attribute__((address_space(3))) mh_s16x4* mh_lds4;
 #define MH_LOG2E 1.4426950408889634f
 #define MH_LN2 0.6931471805599453f
 #define MH_INF __builtin_inff()
+#define MH_GROW 1073741824.f           // 2^30: how far a tile's weights may outgrow the running reference before it is moved
+template <int I> struct MhInt { static constexpr int value = I; };
 
 struct MhaParams {
   const void *q, *k, *v, *o, *d_o;
@@ -41,19 +43,17 @@ struct MhaParams {
 // blockIdx.x -> (unit, tile, split).  Workgroups go round-robin over the 8 XCDs: with a multiple of 8 units (or many) all tiles of a unit get the
 // same residue mod 8, so its keys and values are fetched into ONE XCD's L2.  Otherwise plain order: an uneven share would leave XCDs idle.
 __host__ __device__ inline bool mh_by_xcd(int units) { return units % 8 == 0 || units >= 64; }
+// Causal tiles differ in length: the longest tiles of ALL units come first, so the launch ends with short ones (unit after unit, the last unit's long
+// tiles ran alone at the end: 19 % of the CU time of 64 units x 32 tiles).  Full tiles: unit after unit, so few keys and values are live in an L2 at once.
 __device__ __forceinline__ bool mh_where(const MhaParams& P, int& unit, int& tile, int& split) {
-  const int per = P.tiles * P.splits;
-  int rem;
-  if (mh_by_xcd(P.units)) {
-    const int j = blockIdx.x >> 3;
-    unit = (j / per) * 8 + (blockIdx.x & 7);
-    rem = j % per;
-  } else {
-    unit = blockIdx.x / per;
-    rem = blockIdx.x % per;
-  }
-  tile = rem / P.splits;
-  split = rem % P.splits;
+  const bool x = mh_by_xcd(P.units);
+  const int nu = x ? (P.units + 7) >> 3 : P.units, j = x ? blockIdx.x >> 3 : blockIdx.x;
+  split = j % P.splits;
+  const int k = j / P.splits;
+  int u;
+  if (P.causal) { u = k % nu; tile = k / nu; }
+  else { u = k / P.tiles; tile = k % P.tiles; }
+  unit = x ? u * 8 + (blockIdx.x & 7) : u;
   return unit < P.units;
 }
 static inline long long mh_grid(const MhaParams& P) {
@@ -154,6 +154,10 @@ template <typename T, int NP, int DP, bool WH> __device__ __forceinline__ void m
   }
 }
 
+// Every global load issued so far has arrived.  Placed between the fragment loads of a kernel's prologue and its loop: without it the loop's own waits have to
+// assume that those loads may still be pending, and the first product of EVERY iteration waits for the tile that was only just requested.
+__device__ __forceinline__ void mh_loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }      // vmcnt(0), other counters free
+
 // ---- token-major LDS tile [plane][ROWS][LD] bf16 in 16-byte chunks, chunk c of row r at position c ^ mh_swz(r).  64 banks of 4 bytes: a row read (16 lanes =
 // 16 consecutive rows, one chunk each) and a transposing read (32 lanes = 4 rows x 4 chunks) both touch every bank once.  With rows padded by 16 bytes
 // instead, the four rows of a transposing read overlapped in up to four ways: half of all LDS cycles of the kernels were conflicts.
@@ -218,6 +222,16 @@ template <int NP, int ROWS, int DP> __device__ __forceinline__ void mh_frag_cols
     const mh_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mh_lds4)(a + (r + 8) * LD + (c ^ mh_swz<DP>(r + 8)) * 8));
     const mh_s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     f[p] = __builtin_bit_cast(mh_bf16x8, v);
+  }
+}
+// Order of a product phase of STEPS steps, each with DS LDS reads and MM matrix instructions: the reads run PD steps ahead.  Left to itself the compiler keeps
+// few fragments in flight (read, wait, multiply, read, ...), and every read's ~120 cycles of latency stand between two matrix instructions.
+template <int STEPS, int PD, int DS, int MM> __device__ __forceinline__ void mh_order() {
+  __builtin_amdgcn_sched_group_barrier(0x100, DS * (PD < STEPS ? PD : STEPS), 0);
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, MM, 0);
+    if (i + PD < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, DS, 0);
   }
 }
 // Stores the four channels [c, c + 4) of one token row.

@@ -53,7 +53,7 @@ template <typename T, int DB, bool WH> __device__ __forceinline__ void mh_put(co
 template <typename T, int DP, int KT, int OCC, bool WH>
 __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
   constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, KB = KT / 32;
-  constexpr int TE = MhTile<NP, KT, DP>::ELEMS;
+  constexpr int TE = MhTile<NP, KT, DP>::ELEMS, MM = NP == 3 ? 6 : 1, PD = NP == 3 ? 2 : 4;
   extern __shared__ __attribute__((aligned(16))) unsigned short mh_sm[];       // [2 buffers][K tile | V tile]
   int unit, tile, split;
   if (!mh_where(P, unit, tile, split)) return;
@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
     sv.load(vbase, P.vt, tb * KT, 0, lk);
     sk.store(mh_sm); sv.store(mh_sm + TE);
   }
+  mh_loads_done();
   __syncthreads();
   for (int it = tb; it < te; ++it) {
     const unsigned short* cur = mh_sm + ((it - tb) & 1) * 2 * TE;
@@ -115,6 +116,8 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
           mh_frag_rows<NP, KT, DP>(cur + TE, kb * 32, ks, li, h, A);
           mh_mma<NP>(A, G[ks], E);
         }
+        mh_order<2 * KS, PD, NP, MM>();
+        __builtin_amdgcn_sched_barrier(0);
         const int base = k0 + kb * 32 + 4 * h;
         const bool cut = __any(k0 + kb * 32 + 32 > kmax);
         mh_bf16x8 F[2][NP];
@@ -138,6 +141,8 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
             mh_frag_cols<NP, KT, DP>(cur, kb * 32 + s * 16, d, lane, A);
             mh_mma<NP>(A, F[s], dQ[d]);
           }
+        mh_order<2 * DB, PD, 2 * NP, MM>();
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     if (more) { sk.store(nxt); sv.store(nxt + TE); }
@@ -155,6 +160,7 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
 template <typename T, int DP, int QT, int OCC, bool WH, bool KL>
 __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
   constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, QB = QT / 32;
+  constexpr int MM = NP == 3 ? 6 : 1, PD = NP == 3 ? 2 : 4;
   constexpr int TE = MhTile<NP, QT, DP>::ELEMS, BUF = 2 * TE + 4 * QT;         // Q tile | dO tile | lse2[QT], delta[QT] (floats)
   extern __shared__ __attribute__((aligned(16))) unsigned short mh_sm[];
   int unit, tile, split;
@@ -211,6 +217,7 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
   };
   int ct = lt;                                                                 // query tile of the pair being multiplied
   if (ib < ie) { load(); store(mh_sm); }
+  mh_loads_done();
   __syncthreads();
   for (int it = ib; it < ie; ++it) {
     const unsigned short* cur = mh_sm + ((it - ib) & 1) * BUF;
@@ -240,6 +247,17 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
         mh_frag_rows<NP, QT, DP>(cur + TE, qb * 32, ks, li, h, A);
         mh_mma<NP>(A, V[ks], E);
       }
+      if constexpr (KL) {                                                      // two reads (fragment and K) for every first, one for every second product
+        __builtin_amdgcn_sched_group_barrier(0x100, 3 * NP * 2, 0);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 2 * MM, 0);
+          if (i + 2 < KS) __builtin_amdgcn_sched_group_barrier(0x100, 3 * NP, 0);
+        }
+      } else {
+        mh_order<2 * KS, PD, NP, MM>();
+      }
+      __builtin_amdgcn_sched_barrier(0);
       const bool cut = P.causal && qa + off < kw + 31;
       mh_bf16x8 FP[2][NP], FS[2][NP];
 #pragma unroll
@@ -274,6 +292,8 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
           mh_frag_cols<NP, QT, DP>(cur, qb * 32 + s * 16, d, lane, A);
           mh_mma<NP>(A, FS[s], dK[d]);
         }
+      mh_order<4 * DB, PD, 2 * NP, MM>();
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (more) store(nxt);
     __syncthreads();

@@ -13,7 +13,7 @@
 template <typename T, int DP, int QB, int KT, int OCC, bool WH>
 __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
   constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, KB = KT / 32;
-  constexpr int TE = MhTile<NP, KT, DP>::ELEMS;
+  constexpr int TE = MhTile<NP, KT, DP>::ELEMS, MM = NP == 3 ? 6 : 1, PD = NP == 3 ? 2 : 4;
   extern __shared__ __attribute__((aligned(16))) unsigned short mh_sm[];       // [2 buffers][K tile | V tile]
   int unit, tile, split;
   if (!mh_where(P, unit, tile, split)) return;
@@ -54,14 +54,27 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
   for (int a = 0; a < QB; ++a) kwave = max(kwave, kmax[a]);
 
   mh_f32x16 O[QB][DB];
-  float m[QB], l[QB];
+  float m[QB], ms[QB], l[QB];                                                 // reference (log2) so far, the same with 0 for -inf, sum of 2^(t - ms)
 #pragma unroll
   for (int a = 0; a < QB; ++a) {
-    m[a] = -MH_INF; l[a] = 0.f;
+    m[a] = -MH_INF; ms[a] = 0.f; l[a] = 0.f;
 #pragma unroll
     for (int d = 0; d < DB; ++d) mh_zero(O[a][d]);
   }
 
+  auto weights = [&](const mh_f32x16 (&S)[KB], float ref, mh_bf16x8 (&F)[KB][2][NP]) {
+    float sum = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][s * 8 + j], P.sc2, -ref)); sum += e[j]; }
+        mh_planes<NP>(e, F[kb][s]);
+      }
+    return sum;
+  };
   MhStage<T, NP, KT, DP, WH> sk, sv;
   sk.init(P.kt, P.D); sv.init(P.vt, P.D);
   if (tb < te) {
@@ -69,10 +82,13 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
     sv.load(vbase, P.vt, tb * KT, 0, lk);
     sk.store(mh_sm); sv.store(mh_sm + TE);
   }
+  mh_loads_done();
   __syncthreads();
-  for (int it = tb; it < te; ++it) {
-    const unsigned short* cur = mh_sm + ((it - tb) & 1) * 2 * TE;
-    unsigned short* nxt = mh_sm + (((it - tb) & 1) ^ 1) * 2 * TE;
+  // One key tile: BUF (which buffer it lies in) is a constant, so every LDS address below is one register and an immediate.
+  auto step = [&](auto buf_, int it) {
+    constexpr int BUF = decltype(buf_)::value;
+    const unsigned short* cur = mh_sm + BUF * 2 * TE;
+    unsigned short* nxt = mh_sm + (BUF ^ 1) * 2 * TE;
     const bool more = it + 1 < te;
     if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk); }
     const int k0 = it * KT;
@@ -90,6 +106,8 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
           for (int a = 0; a < QB; ++a) mh_mma<NP>(A, Q[a][ks], S[a][kb]);
         }
       }
+      mh_order<KB * KS, PD, NP, MM * QB>();
+      __builtin_amdgcn_sched_barrier(0);
       mh_bf16x8 F[QB][KB][2][NP];
 #pragma unroll
       for (int a = 0; a < QB; ++a) {
@@ -97,32 +115,28 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) mh_mask_keys(S[a][kb], k0 + kb * 32 + 4 * h, kmax[a]);
         }
-        float mx = S[a][0][0];
+        // p = 2^(t - ms) with the reference ms of the tiles before: fp32 and bf16 share their exponent range, so ms only has to be NEAR the maximum.  It
+        // moves (below) when a column has seen no key yet or a tile outgrows it by MH_GROW, which leaves three instructions a score here.
+        float sum = weights(S[a], ms[a], F[a]);
+        if (__any(m[a] == -MH_INF || !(sum <= MH_GROW))) {
+          float mx = S[a][0][0];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+          for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[a][kb][r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m[a], mx * P.sc2), ms = mn == -MH_INF ? 0.f : mn;      // a column that has seen no key yet keeps p = 2^-inf = 0
-        const float al = __builtin_amdgcn_exp2f(m[a] - ms);
-        m[a] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            float e[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) { e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[a][kb][s * 8 + j], P.sc2, -ms)); sum += e[j]; }
-            mh_planes<NP>(e, F[a][kb][s]);
-          }
-        l[a] = l[a] * al + sum;
-        if (__any(al != 1.f)) {
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[a][kb][r]);
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          const float mn = fmaxf(m[a], mx * P.sc2);
+          ms[a] = mn == -MH_INF ? 0.f : mn;                                    // a column that has seen no key yet keeps p = 2^-inf = 0
+          const float al = __builtin_amdgcn_exp2f(m[a] - ms[a]);
+          m[a] = mn;
+          sum = weights(S[a], ms[a], F[a]);
+          l[a] *= al;
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) O[a][d][r] *= al;
         }
+        l[a] += sum;
       }
 #pragma unroll
       for (int d = 0; d < DB; ++d)
@@ -135,9 +149,14 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
 #pragma unroll
             for (int a = 0; a < QB; ++a) mh_mma<NP>(A, F[a][kb][s], O[a][d]);
           }
+      mh_order<DB * KB * 2, PD, 2 * NP, MM * QB>();
     }
     if (more) { sk.store(nxt); sv.store(nxt + TE); }
     __syncthreads();
+  };
+  for (int it = tb; it < te; it += 2) {
+    step(MhInt<0>(), it);
+    if (it + 1 < te) step(MhInt<1>(), it + 1);
   }
 
 #pragma unroll

@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
   MhStage<T, NP, KT, DP, WH> sk, sv;
   sk.init(P.kt, P.D); sv.init(P.vt, P.D);
   if (tb < te) {
-    sk.load(kbase, P.kt, tb * KT, 0, lk);
-    sv.load(vbase, P.vt, tb * KT, 0, lk);
+    sk.load(kbase, P.kt, tb * KT, 0, lk, mh_sm);
+    sv.load(vbase, P.vt, tb * KT, 0, lk, mh_sm + TE);
     sk.store(mh_sm); sv.store(mh_sm + TE);
   }
   mh_loads_done();
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
     const unsigned short* cur = mh_sm + ((it - tb) & 1) * 2 * TE;
     unsigned short* nxt = mh_sm + (((it - tb) & 1) ^ 1) * 2 * TE;
     const bool more = it + 1 < te;
-    if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk); }
+    if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk, nxt); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk, nxt + TE); }
     const int k0 = it * KT;
     if (wlive && __any(kmax > k0)) {
 #pragma unroll
@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
       }
     }
     if (more) { sk.store(nxt); sv.store(nxt + TE); }
+    mh_arrive<decltype(sk)::DMA>();
     __syncthreads();
   }
   if (tq >= P.Tq) return;
@@ -161,7 +162,7 @@ template <typename T, int DP, int QT, int OCC, bool WH, bool KL>
 __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
   constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, QB = QT / 32;
   constexpr int MM = NP == 3 ? 6 : 1, PD = NP == 3 ? 2 : 4;
-  constexpr int TE = MhTile<NP, QT, DP>::ELEMS, BUF = 2 * TE + 4 * QT;         // Q tile | dO tile | lse2[QT], delta[QT] (floats)
+  constexpr int TE = MhTile<NP, QT, DP>::ELEMS, BUF = 2 * TE + 4 * QT;         // Q tile | dO tile | -lse2[QT], -delta[QT] (floats)
   extern __shared__ __attribute__((aligned(16))) unsigned short mh_sm[];
   int unit, tile, split;
   if (!mh_where(P, unit, tile, split)) return;
@@ -197,33 +198,41 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
   MhStage<T, NP, QT, DP, WH> sq, sg;
   sq.init(P.qt, P.D); sg.init(P.ot, P.D);
   float rl = 0.f, rd = 0.f;
-  auto load = [&]() {
+  bool rin = false;
+  auto load = [&](unsigned short* buf) {
     const int hq = hk * P.G + lh, q0 = (q0t + lt) * QT;
-    sq.load((const T*)P.q + b * P.qb + (long long)hq * P.qh, P.qt, q0, qlo, lq);
-    sg.load((const T*)P.d_o + b * P.ob + (long long)hq * P.oh, P.ot, q0, qlo, lq);
-    // rows that do not count come as lse = +inf: their probabilities are exact zeros
+    sq.load((const T*)P.q + b * P.qb + (long long)hq * P.qh, P.qt, q0, qlo, lq, buf);
+    sg.load((const T*)P.d_o + b * P.ob + (long long)hq * P.oh, P.ot, q0, qlo, lq, buf + TE);
     const int tq = q0 + (t & (QT - 1));
-    const bool in = tq >= qlo && tq < lq;
-    const long long i = ((long long)b * P.Hq + hq) * P.Tq + (in ? tq : 0);
-    const float e = P.lse[i], d = P.delta[i];
-    rl = !in || e == -MH_INF ? MH_INF : e * MH_LOG2E;
-    rd = in ? d : 0.f;
+    rin = tq >= qlo && tq < lq;
+    const long long i = ((long long)b * P.Hq + hq) * P.Tq + (rin ? tq : 0);
+    rl = P.lse[i]; rd = P.delta[i];                                            // (looked at in store(): here it would wait for the loads)
     if (++lt == nq) { lt = 0; ++lh; }
   };
   auto store = [&](unsigned short* buf) {
     sq.store(buf); sg.store(buf + TE);
     float* st = reinterpret_cast<float*>(buf + 2 * TE);
-    if (t < QT) { st[t] = rl; st[QT + t] = rd; }
+    // rows that do not count come as -lse = -inf: their probabilities are exact zeros
+    if (t < QT) { st[t] = !rin || rl == -MH_INF ? -MH_INF : rl * -MH_LOG2E; st[QT + t] = rin ? -rd : 0.f; }
   };
   int ct = lt;                                                                 // query tile of the pair being multiplied
-  if (ib < ie) { load(); store(mh_sm); }
+  if (ib < ie) { load(mh_sm); store(mh_sm); }
   mh_loads_done();
   __syncthreads();
+  // the statistics of a lane's 16 rows: 8 g + 4 h ..+3 for g = 0..3
+  auto stat = [&](const float* st, mh_f32x16& v) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const tk_f32x4 x = *reinterpret_cast<const tk_f32x4*>(st + 8 * g + 4 * h);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[g * 4 + j] = x[j];
+    }
+  };
   for (int it = ib; it < ie; ++it) {
     const unsigned short* cur = mh_sm + ((it - ib) & 1) * BUF;
     unsigned short* nxt = mh_sm + (((it - ib) & 1) ^ 1) * BUF;
     const bool more = it + 1 < ie;
-    if (more) load();
+    if (more) load(nxt);
     const int q0 = (q0t + ct) * QT;
     if (++ct == nq) ct = 0;
     const float* st = reinterpret_cast<const float*>(cur + 2 * TE);
@@ -231,7 +240,8 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
     for (int qb = 0; qb < QB; ++qb) {
       const int qa = q0 + qb * 32;
       mh_f32x16 S, E;
-      mh_zero(S); mh_zero(E);
+      mh_zero(S);
+      stat(st + QT + qb * 32, E);                                              // dP - delta: the accumulator starts at -delta
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         mh_bf16x8 A[NP];
@@ -248,36 +258,35 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
         mh_mma<NP>(A, V[ks], E);
       }
       if constexpr (KL) {                                                      // two reads (fragment and K) for every first, one for every second product
-        __builtin_amdgcn_sched_group_barrier(0x100, 3 * NP * 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4 + 3 * NP * 2, 0);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 2 * MM, 0);
           if (i + 2 < KS) __builtin_amdgcn_sched_group_barrier(0x100, 3 * NP, 0);
         }
       } else {
-        mh_order<2 * KS, PD, NP, MM>();
+        mh_order<2 * KS, PD, NP, MM, 4>();
       }
       __builtin_amdgcn_sched_barrier(0);
-      const bool cut = P.causal && qa + off < kw + 31;
+      if (P.causal && qa + off < kw + 31) {                                    // a pair above the diagonal is in the block (uniform)
+        asm volatile("");                                                      // (a branch, not selects in every block)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool see = qa + 4 * h + (r & 3) + 8 * (r >> 2) + off >= key;
+          S[r] = see ? S[r] : -MH_INF; E[r] = see ? E[r] : 0.f;
+        }
+      }
+      mh_f32x16 L;
       mh_bf16x8 FP[2][NP], FS[2][NP];
+      stat(st + qb * 32, L);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float p[8], e[8];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {                                          // four consecutive queries: rows 8 (2 s + g) + 4 h ..+3
-          const tk_f32x4 l4 = *reinterpret_cast<const tk_f32x4*>(st + qb * 32 + 8 * (2 * s + g) + 4 * h);
-          const tk_f32x4 d4 = *reinterpret_cast<const tk_f32x4*>(st + QT + qb * 32 + 8 * (2 * s + g) + 4 * h);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = s * 8 + g * 4 + j;
-            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], P.sc2, -l4[j]));
-            float y = x * (E[r] - d4[j]);
-            if (cut) {
-              const bool see = qa + 8 * (2 * s + g) + 4 * h + j + off >= key;
-              x = see ? x : 0.f; y = see ? y : 0.f;
-            }
-            p[g * 4 + j] = x; e[g * 4 + j] = y;
-          }
+        for (int j = 0; j < 8; ++j) {
+          const int r = s * 8 + j;
+          p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], P.sc2, L[r]));
+          e[j] = p[j] * E[r];
         }
         mh_planes<NP>(p, FP[s]);
         mh_planes<NP>(e, FS[s]);
@@ -292,10 +301,11 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
           mh_frag_cols<NP, QT, DP>(cur, qb * 32 + s * 16, d, lane, A);
           mh_mma<NP>(A, FS[s], dK[d]);
         }
-      mh_order<4 * DB, PD, 2 * NP, MM>();
+      mh_order<4 * DB, PD, 2 * NP, MM, 4>();
       __builtin_amdgcn_sched_barrier(0);
     }
     if (more) store(nxt);
+    mh_arrive<decltype(sq)::DMA>();
     __syncthreads();
   }
   if (key >= P.Tk) return;

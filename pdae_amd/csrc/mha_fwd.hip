@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
     for (int d = 0; d < DB; ++d) mh_zero(O[a][d]);
   }
 
-  auto weights = [&](const mh_f32x16 (&S)[KB], float ref, mh_bf16x8 (&F)[KB][2][NP]) {
+  auto weights = [&](const mh_f32x16 (&S)[KB], float ref, mh_bf16x8 (&F)[KB][2][NP]) __attribute__((always_inline)) {
     float sum = 0.f;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -78,19 +78,19 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
   MhStage<T, NP, KT, DP, WH> sk, sv;
   sk.init(P.kt, P.D); sv.init(P.vt, P.D);
   if (tb < te) {
-    sk.load(kbase, P.kt, tb * KT, 0, lk);
-    sv.load(vbase, P.vt, tb * KT, 0, lk);
+    sk.load(kbase, P.kt, tb * KT, 0, lk, mh_sm);
+    sv.load(vbase, P.vt, tb * KT, 0, lk, mh_sm + TE);
     sk.store(mh_sm); sv.store(mh_sm + TE);
   }
   mh_loads_done();
   __syncthreads();
   // One key tile: BUF (which buffer it lies in) is a constant, so every LDS address below is one register and an immediate.
-  auto step = [&](auto buf_, int it) {
+  auto step = [&](auto buf_, int it) __attribute__((always_inline)) {
     constexpr int BUF = decltype(buf_)::value;
     const unsigned short* cur = mh_sm + BUF * 2 * TE;
     unsigned short* nxt = mh_sm + (BUF ^ 1) * 2 * TE;
     const bool more = it + 1 < te;
-    if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk); }
+    if (more) { sk.load(kbase, P.kt, (it + 1) * KT, 0, lk, nxt); sv.load(vbase, P.vt, (it + 1) * KT, 0, lk, nxt + TE); }
     const int k0 = it * KT;
     if (wlive && __any(kwave > k0)) {
       mh_f32x16 S[QB][KB];
@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
       mh_order<DB * KB * 2, PD, 2 * NP, MM * QB>();
     }
     if (more) { sk.store(nxt); sv.store(nxt + TE); }
+    mh_arrive<decltype(sk)::DMA>();
     __syncthreads();
   };
   for (int it = tb; it < te; it += 2) {

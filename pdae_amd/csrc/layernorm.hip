@@ -2,8 +2,8 @@
 //     g = dy gamma;  dx = rstd (g - mean(g) - xh mean(g xh)) (+ add);  dgamma = sum_rows dy xh;  dbeta = sum_rows dy,   xh = (x - mu) rstd.
 //
 // Bound: HBM (forward one read and one write of the tensor, backward two reads and one write).  A row is read ONCE and lives in registers between its
-// reductions: a wave owns a row (WPR = 1: short rows, four rows a block, no barrier) or the block's four waves share it (WPR = 4).  NV vectors of eight
-// elements a lane; rows longer than 4 * 64 * 8 * 8 = 16384 channels are streamed from L2 a second and third time (NV = 0).
+// reductions: L lanes share it (8 .. 64 of a wave, or a block of 256 / 512), NV vectors of eight elements a lane; only rows beyond 16384 channels are
+// streamed again from L2 (NV = 0).  65536 x 1536 bf16: forward 78 us, backward 135 us (5.2 / 4.5 TB/s; a large copy on this chip moves 5.2).
 // The variance is taken from the deviations (two passes over registers), not from E[x^2] - E[x]^2, which loses what a large mean leaves.
 //
 // Weight gradients: every block walks a fixed set of rows and keeps sum dy xh / sum dy of its lanes' own channels in registers; it leaves ONE partial row per
@@ -11,30 +11,31 @@
 #include "token.h"
 #include "kernels.h"
 
-#define LN_T 256
-#define LN_MAXB 1024           // partial rows of the weight gradients (blocks of the backward launch)
 
-template <int WPR> __device__ __forceinline__ float ln_sum(float v, float* red) {
+// sum over the L lanes that share a row (L <= 64: neighbouring lanes of a wave; else the whole block of L threads)
+template <int L> __device__ __forceinline__ float ln_sum(float v, float* red) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-  if constexpr (WPR == 4) {
+  for (int off = (L < 64 ? L : 64) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off);
+  if constexpr (L > 64) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = (red[0] + red[1]) + (red[2] + red[3]);
+    if constexpr (L == 512) v += (red[4] + red[5]) + (red[6] + red[7]);
   }
   return v;
 }
+#define LN_THREADS(L) ((L) > 256 ? (L) : 256)
 
 // Elements of a row: nv = C / 8 whole vectors (vector i of lane `lane` is number lane + i * lanes) and C % 8 single elements on the first lanes.
-template <typename T, int WPR, int NV>
-__global__ void __launch_bounds__(LN_T) layernorm_fwd_kernel(const T* __restrict__ x, long long ldx, const float* __restrict__ gamma,
+template <typename T, int L, int NV>
+__global__ void __launch_bounds__(LN_THREADS(L)) layernorm_fwd_kernel(const T* __restrict__ x, long long ldx, const float* __restrict__ gamma,
                                                              const float* __restrict__ beta, int R, int C, float eps, T* __restrict__ y, long long ldy,
                                                              float* __restrict__ mean, float* __restrict__ rstd) {
-  __shared__ float red[4];
-  constexpr int LANES = 64 * WPR, RPB = 4 / WPR;
-  const int lane = threadIdx.x % LANES, row = blockIdx.x * RPB + threadIdx.x / LANES;
-  if (row >= R) return;                                    // WPR == 4: never (one row a block)
+  __shared__ float red[8];
+  constexpr int RPB = LN_THREADS(L) / L;
+  const int lane = threadIdx.x % L, row = blockIdx.x * RPB + threadIdx.x / L;
+  if (row >= R) return;                                    // (whole lane groups; L > 64: never, one row a block)
   const int nv = C >> 3, tail = C & 7, te = nv * 8 + lane;
   const T* xr = x + (long long)row * ldx;
   T* yr = y + (long long)row * ldy;
@@ -46,7 +47,7 @@ __global__ void __launch_bounds__(LN_T) layernorm_fwd_kernel(const T* __restrict
   if constexpr (NV > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = lane + i * LANES;
+      const int c = lane + i * L;
       if (c < nv) TkVec<T>::load8(xr + c * 8, v[i]);
       else {
 #pragma unroll
@@ -56,29 +57,29 @@ __global__ void __launch_bounds__(LN_T) layernorm_fwd_kernel(const T* __restrict
       for (int j = 0; j < 8; ++j) s += v[i][j];
     }
   } else {
-    for (int c = lane; c < nv; c += LANES) {
+    for (int c = lane; c < nv; c += L) {
       TkVec<T>::load8(xr + c * 8, v[0]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += v[0][j];
     }
   }
-  const float mu = ln_sum<WPR>(s, red) / n;
+  const float mu = ln_sum<L>(s, red) / n;
   float q = has ? (xt - mu) * (xt - mu) : 0.f;
   if constexpr (NV > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (lane + i * LANES < nv) {
+      if (lane + i * L < nv) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) { const float d = v[i][j] - mu; q += d * d; }
       }
   } else {
-    for (int c = lane; c < nv; c += LANES) {
+    for (int c = lane; c < nv; c += L) {
       TkVec<T>::load8(xr + c * 8, v[0]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) { const float d = v[0][j] - mu; q += d * d; }
     }
   }
-  const float rs = 1.0f / sqrtf(ln_sum<WPR>(q, red) / n + eps);
+  const float rs = 1.0f / sqrtf(ln_sum<L>(q, red) / n + eps);
   if (lane == 0) {
     if (mean) mean[row] = mu;
     if (rstd) rstd[row] = rs;
@@ -94,145 +95,211 @@ __global__ void __launch_bounds__(LN_T) layernorm_fwd_kernel(const T* __restrict
   if constexpr (NV > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (lane + i * LANES < nv) emit(lane + i * LANES, v[i]);
+      if (lane + i * L < nv) emit(lane + i * L, v[i]);
   } else {
-    for (int c = lane; c < nv; c += LANES) { TkVec<T>::load8(xr + c * 8, v[0]); emit(c, v[0]); }
+    for (int c = lane; c < nv; c += L) { TkVec<T>::load8(xr + c * 8, v[0]); emit(c, v[0]); }
   }
   if (has) TkVec<T>::store(yr + te, (xt - mu) * rs * (gamma ? gamma[te] : 1.f) + (beta ? beta[te] : 0.f));
 }
 
-// part: [gridDim.x][2][C] partial sums of dy xh and dy (written only when WG).  With NV == 0 (streamed rows) the block adds its rows into its own
-// partial row in memory: every channel of it belongs to one lane, so no other thread touches it.
-template <typename T, int WPR, int NV, bool WG>
-__global__ void __launch_bounds__(LN_T) layernorm_bwd_kernel(const T* __restrict__ x, long long ldx, const float* __restrict__ gamma,
+// Eight elements as they lie in memory (four or eight dwords), and as fp32.
+template <typename T> struct LnRaw { unsigned w[sizeof(T) * 2]; };
+template <typename T> __device__ __forceinline__ void ln_read(const T* p, LnRaw<T>& r) { __builtin_memcpy(r.w, p, 8 * sizeof(T)); }
+template <typename T> __device__ __forceinline__ float ln_elem(const LnRaw<T>& r, int j) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[j]);
+  else return __uint_as_float(j & 1 ? r.w[j / 2] & 0xffff0000u : r.w[j / 2] << 16);
+}
+
+// part: [gridDim.x][2][C] partial sums of dy xh and dy (written only when WG).  A row is held as it was read and converted twice (row sums, then dx): its fp32
+// forms would take four times the registers, and the row AFTER it could not be in flight meanwhile -- with one row at a time a wave waited for HBM
+// on every row (65536 x 1536 bf16: 239 us, 2.5 TB/s).
+template <typename T, int L, int NV, bool WG>
+__global__ void __launch_bounds__(LN_THREADS(L)) layernorm_bwd_kernel(const T* __restrict__ x, long long ldx, const float* __restrict__ gamma,
                                                              const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ dy,
                                                              long long lddy, const T* add, long long ldadd, int R, int C, T* dx, long long lddx,
                                                              float* __restrict__ part) {
-  __shared__ float red[8];
-  __shared__ float comb[WPR == 1 && WG && NV > 0 ? 2 * 64 * 9 : 1];
-  constexpr int LANES = 64 * WPR, RPB = 4 / WPR, NR = NV > 0 ? NV : 1;
-  const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+  __shared__ float red[16];
+  __shared__ float comb[L <= 64 && WG ? 2 * L * 9 : 1];
+  constexpr int RPB = LN_THREADS(L) / L;
+  const int lane = threadIdx.x % L, sub = L > 64 ? 0 : L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int)threadIdx.x / L;
   const int nv = C >> 3, tail = C & 7, te = nv * 8 + lane;
-  const float n = (float)C;                                // (divided by, not multiplied with its reciprocal: the mean of a constant row is exact)
+  const float n = (float)C;
   const bool has = lane < tail;
-  float ag[NR][8], ab[NR][8], agt = 0.f, abt = 0.f;
+  float ag[NV][8], ab[NV][8], gm[NV][8], agt = 0.f, abt = 0.f, gmt = 1.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { ag[i][j] = ab[i][j] = 0.f; gm[i][j] = 1.f; }
+    if (gamma && lane + i * L < nv) TkVec<float>::load8(gamma + (lane + i * L) * 8, gm[i]);
+  }
+  if (gamma && has) gmt = gamma[te];
+  LnRaw<T> qx[2][NV], qd[2][NV];
+  float tx[2], td[2], mu[2], rs[2];
+  const long long step = (long long)gridDim.x * RPB;
+  auto fetch = [&](long long row, LnRaw<T> (&rx)[NV], LnRaw<T> (&rd)[NV], float& ex, float& ed, float& m, float& r) __attribute__((always_inline)) {
+    const T* xr = x + row * ldx;
+    const T* dr = dy + row * lddy;
+    m = mean[row]; r = rstd[row];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (lane + i * L < nv) { ln_read(xr + (lane + i * L) * 8, rx[i]); ln_read(dr + (lane + i * L) * 8, rd[i]); }
+      else {
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(T) * 2); ++j) rx[i].w[j] = rd[i].w[j] = 0;
+      }
+    ex = has ? TkVec<T>::load(xr + te) : 0.f;
+    ed = has ? TkVec<T>::load(dr + te) : 0.f;
+  };
+  auto work = [&](long long row, LnRaw<T> (&rx)[NV], LnRaw<T> (&rd)[NV], float ex, float ed, float m, float r) __attribute__((always_inline)) {
+    float s1 = 0.f, s2 = 0.f;
+    float xt = 0.f, gt = 0.f;
+    if (has) {
+      xt = (ex - m) * r; gt = ed * gmt;
+      s1 = gt; s2 = gt * xt;
+      agt += ed * xt; abt += ed;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (lane + i * L < nv) {                          // (lanes past the row's end hold zeros, but (0 - mu) rstd is none)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float xh = (ln_elem(rx[i], j) - m) * r, d = ln_elem(rd[i], j), g = d * gm[i][j];
+          if (WG) { ag[i][j] += d * xh; ab[i][j] += d; }
+          s1 += g; s2 += g * xh;
+        }
+      }
+    const float m1 = ln_sum<L>(s1, red) / n, m2 = ln_sum<L>(s2, red + 8) / n;
+    const T* ar = add ? add + row * ldadd : nullptr;
+    T* orow = dx + row * lddx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (lane + i * L < nv) {
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(T) * 2); ++j) { asm volatile("" : "+v"(rx[i].w[j])); asm volatile("" : "+v"(rd[i].w[j])); }      // convert anew, do not keep
+        const int c = (lane + i * L) * 8;
+        float o[8], e[8];
+        if (ar) TkVec<T>::load8(ar + c, e);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float xh = (ln_elem(rx[i], j) - m) * r, g = ln_elem(rd[i], j) * gm[i][j];
+          o[j] = r * (g - m1 - xh * m2);
+          if (ar) o[j] += e[j];
+        }
+        TkVec<T>::store8(orow + c, o);
+      }
+    if (has) TkVec<T>::store(orow + te, r * (gt - m1 - xt * m2) + (ar ? TkVec<T>::load(ar + te) : 0.f));
+  };
+  // two rows in turn, the next one in flight while this one is worked on (L > 64: all waves of the block walk the same rows)
+  const long long row0 = (long long)blockIdx.x * RPB + sub;
+  if (row0 < R) fetch(row0, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
+  for (long long row = row0; row < R; row += 2 * step) {
+    if (row + step < R) fetch(row + step, qx[1], qd[1], tx[1], td[1], mu[1], rs[1]);
+    work(row, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
+    if (row + 2 * step < R) fetch(row + 2 * step, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
+    if (row + step < R) work(row + step, qx[1], qd[1], tx[1], td[1], mu[1], rs[1]);
+  }
+  if constexpr (WG) {
+    float* pg = part + (size_t)blockIdx.x * 2 * C;
+    float* pb = pg + C;
+    if constexpr (L > 64) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (lane + i * L < nv) { TkVec<float>::store8(pg + (lane + i * L) * 8, ag[i]); TkVec<float>::store8(pb + (lane + i * L) * 8, ab[i]); }
+      if (has) { pg[te] = agt; pb[te] = abt; }
+    } else {
+      // first the lane groups of a wave, then the four waves in wave order through LDS, a vector at a time
+      const int w = threadIdx.x >> 6;
+#pragma unroll
+      for (int off = L; off < 64; off <<= 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) { ag[i][j] += __shfl_xor(ag[i][j], off); ab[i][j] += __shfl_xor(ab[i][j], off); }
+        agt += __shfl_xor(agt, off); abt += __shfl_xor(abt, off);
+      }
+      const bool mine = (threadIdx.x & 63) < L;
+#pragma unroll
+      for (int i = 0; i <= NV; ++i) {                       // i == NV: the C % 8 single channels
+        for (int k = 0; k < 4; ++k) {
+          if (w == k && mine) {
+            float* c0 = comb + lane * 9;
+            float* c1 = comb + (L + lane) * 9;
+#pragma unroll
+            for (int j = 0; j < (i < NV ? 8 : 1); ++j) {
+              const float g = i < NV ? ag[i < NV ? i : 0][j] : agt, b = i < NV ? ab[i < NV ? i : 0][j] : abt;
+              c0[j] = k ? c0[j] + g : g; c1[j] = k ? c1[j] + b : b;
+            }
+            if (k == 3 && i < NV && lane + i * L < nv) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) { pg[(lane + i * L) * 8 + j] = c0[j]; pb[(lane + i * L) * 8 + j] = c1[j]; }
+            }
+            if (k == 3 && i == NV && has) { pg[te] = c0[0]; pb[te] = c1[0]; }
+          }
+          __syncthreads();
+        }
+      }
+    }
+  }
+}
+
+// Rows too long for registers: the block reads its row twice (the second time from L2) and adds into its own partial row in memory; every channel of
+// it belongs to one lane, so no other thread touches it.
+template <typename T, bool WG>
+__global__ void __launch_bounds__(512) layernorm_bwd_long_kernel(const T* __restrict__ x, long long ldx, const float* __restrict__ gamma,
+                                                                 const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ dy,
+                                                                 long long lddy, const T* add, long long ldadd, int R, int C, T* dx, long long lddx,
+                                                                 float* __restrict__ part) {
+  __shared__ float red[16];
+  const float n = (float)C;
+  const int t = threadIdx.x, nv = C >> 3, te = nv * 8 + t;
+  const bool has = t < (C & 7);
   float* pg = part + (size_t)blockIdx.x * 2 * C;
   float* pb = pg + C;
-  if constexpr (NV > 0) {
-#pragma unroll
-    for (int i = 0; i < NR; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ag[i][j] = ab[i][j] = 0.f;
-  } else if constexpr (WG) {
-    const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int c = lane; c < nv; c += LANES) { TkVec<float>::store8(pg + c * 8, z); TkVec<float>::store8(pb + c * 8, z); }
-  }
-  for (long long row0 = (long long)blockIdx.x * RPB; row0 < R; row0 += (long long)gridDim.x * RPB) {
-    const long long row = row0 + sub;
-    if (row >= R) break;                                   // WPR == 4: never (whole blocks)
+  for (long long row = blockIdx.x; row < R; row += gridDim.x) {
     const T* xr = x + row * ldx;
     const T* dr = dy + row * lddy;
     const T* ar = add ? add + row * ldadd : nullptr;
-    T* or_ = dx + row * lddx;
+    T* orow = dx + row * lddx;
     const float mu = mean[row], rs = rstd[row];
-    float xh[NR][8], g[NR][8];
+    const bool one = row == blockIdx.x;                    // the partial row starts with the block's first row
     float s1 = 0.f, s2 = 0.f, xt = 0.f, gt = 0.f;
     if (has) {
       const float d = TkVec<T>::load(dr + te);
       xt = (TkVec<T>::load(xr + te) - mu) * rs;
       gt = gamma ? d * gamma[te] : d;
       s1 = gt; s2 = gt * xt;
-      agt += d * xt; abt += d;
+      if (WG) { pg[te] = one ? d * xt : pg[te] + d * xt; pb[te] = one ? d : pb[te] + d; }
     }
-    auto take = [&](int c, float (&xv)[8], float (&gv)[8]) {          // xv: xh, gv: dy gamma; returns with the row sums updated
-      TkVec<T>::load8(xr + c * 8, xv);
-      TkVec<T>::load8(dr + c * 8, gv);
-    };
-    auto weigh = [&](int c, float (&xv)[8], float (&gv)[8], float* accg, float* accb) {
-      float gm[8];
+    for (int c = t; c < nv; c += 512) {
+      float xh[8], d[8], gm[8], p[8], q[8];
+      TkVec<T>::load8(xr + c * 8, xh);
+      TkVec<T>::load8(dr + c * 8, d);
       if (gamma) TkVec<float>::load8(gamma + c * 8, gm);
+      if (WG && !one) { TkVec<float>::load8(pg + c * 8, p); TkVec<float>::load8(pb + c * 8, q); }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        xv[j] = (xv[j] - mu) * rs;
-        if (WG) { accg[j] += gv[j] * xv[j]; accb[j] += gv[j]; }
-        if (gamma) gv[j] *= gm[j];
-        s1 += gv[j]; s2 += gv[j] * xv[j];
+        xh[j] = (xh[j] - mu) * rs;
+        p[j] = (one ? 0.f : p[j]) + d[j] * xh[j]; q[j] = (one ? 0.f : q[j]) + d[j];
+        const float g = gamma ? d[j] * gm[j] : d[j];
+        s1 += g; s2 += g * xh[j];
       }
-    };
-    if constexpr (NV > 0) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (lane + i * LANES < nv) take(lane + i * LANES, xh[i], g[i]);
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (lane + i * LANES < nv) weigh(lane + i * LANES, xh[i], g[i], ag[i], ab[i]);
-    } else {
-      for (int c = lane; c < nv; c += LANES) {
-        float pgv[8], pbv[8];
-        take(c, xh[0], g[0]);
-        if (WG) { TkVec<float>::load8(pg + c * 8, pgv); TkVec<float>::load8(pb + c * 8, pbv); }
-        weigh(c, xh[0], g[0], pgv, pbv);
-        if (WG) { TkVec<float>::store8(pg + c * 8, pgv); TkVec<float>::store8(pb + c * 8, pbv); }
-      }
+      if (WG) { TkVec<float>::store8(pg + c * 8, p); TkVec<float>::store8(pb + c * 8, q); }
     }
-    const float m1 = ln_sum<WPR>(s1, red) / n, m2 = ln_sum<WPR>(s2, red + 4) / n;
-    auto emit = [&](int c, const float (&xv)[8], const float (&gv)[8]) {
-      float o[8], a[8];
-      if (ar) TkVec<T>::load8(ar + c * 8, a);
+    const float m1 = ln_sum<512>(s1, red) / n, m2 = ln_sum<512>(s2, red + 8) / n;
+    for (int c = t; c < nv; c += 512) {
+      float xh[8], d[8], gm[8], e[8], o[8];
+      TkVec<T>::load8(xr + c * 8, xh);
+      TkVec<T>::load8(dr + c * 8, d);
+      if (gamma) TkVec<float>::load8(gamma + c * 8, gm);
+      if (ar) TkVec<T>::load8(ar + c * 8, e);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { o[j] = rs * (gv[j] - m1 - xv[j] * m2); if (ar) o[j] += a[j]; }
-      TkVec<T>::store8(or_ + c * 8, o);
-    };
-    if constexpr (NV > 0) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (lane + i * LANES < nv) emit(lane + i * LANES, xh[i], g[i]);
-    } else {
-      for (int c = lane; c < nv; c += LANES) {
-        float gm[8];
-        take(c, xh[0], g[0]);
-        if (gamma) TkVec<float>::load8(gamma + c * 8, gm);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { xh[0][j] = (xh[0][j] - mu) * rs; if (gamma) g[0][j] *= gm[j]; }
-        emit(c, xh[0], g[0]);
+      for (int j = 0; j < 8; ++j) {
+        o[j] = rs * ((gamma ? d[j] * gm[j] : d[j]) - m1 - (xh[j] - mu) * rs * m2);
+        if (ar) o[j] += e[j];
       }
+      TkVec<T>::store8(orow + c * 8, o);
     }
-    if (has) TkVec<T>::store(or_ + te, rs * (gt - m1 - xt * m2) + (ar ? TkVec<T>::load(ar + te) : 0.f));
-  }
-  if constexpr (WG) {
-    if constexpr (WPR == 4) {
-      if constexpr (NV > 0) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (lane + i * LANES < nv) { TkVec<float>::store8(pg + (lane + i * LANES) * 8, ag[i]); TkVec<float>::store8(pb + (lane + i * LANES) * 8, ab[i]); }
-      }
-      if (has) { pg[te] = agt; pb[te] = abt; }
-    } else {                                               // four waves, one partial row: added in wave order through LDS, a vector at a time
-#pragma unroll
-      for (int i = 0; i < NR; ++i) {
-        for (int w = 0; w < 4; ++w) {
-          if (sub == w) {
-            float* c0 = comb + lane * 9;
-            float* c1 = comb + (64 + lane) * 9;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) { c0[j] = w ? c0[j] + ag[i][j] : ag[i][j]; c1[j] = w ? c1[j] + ab[i][j] : ab[i][j]; }
-            if (w == 3 && lane + i * 64 < nv) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) { pg[(lane + i * 64) * 8 + j] = c0[j]; pb[(lane + i * 64) * 8 + j] = c1[j]; }
-            }
-          }
-          __syncthreads();
-        }
-      }
-      for (int w = 0; w < 4; ++w) {
-        if (sub == w) {
-          comb[lane * 9] = w ? comb[lane * 9] + agt : agt;
-          comb[(64 + lane) * 9] = w ? comb[(64 + lane) * 9] + abt : abt;
-          if (w == 3 && has) { pg[te] = comb[lane * 9]; pb[te] = comb[(64 + lane) * 9]; }
-        }
-        __syncthreads();
-      }
-    }
+    if (has) TkVec<T>::store(orow + te, rs * (gt - m1 - xt * m2) + (ar ? TkVec<T>::load(ar + te) : 0.f));
   }
 }
 
@@ -257,50 +324,69 @@ __global__ void __launch_bounds__(1024) layernorm_wsum_kernel(const float* __res
   }
 }
 
-// Row form by length: one wave a row while it fits 4 vectors a lane (2048 channels), else four waves a row up to 8 vectors, else streamed.
-struct LnForm { int wpr, nv; };
-static LnForm ln_form(int C) {
+// Row form: the smallest group of lanes that holds a row in one vector each (8, 16, 32 or a whole wave up to 512 channels: 64-channel rows on whole
+// waves ran at 0.75 TB/s, seven lanes of eight idle), a wave up to 4 vectors a lane (2048 channels; backward, which keeps more state: 3), then four
+// waves, eight waves (16384 channels), streamed beyond.  Few rows (fewer blocks than CUs at four rows a block) go to four waves each: 128 rows of
+// 2048 fp32, one layer of a latent batch, took 5.0 + 8.6 us with one wave a row, 4.0 + 4.9 with four.
+struct LnForm { int lanes, nv; };
+static LnForm ln_form(int R, int C, bool bwd) {
   const int nv = C / 8;
-  if (nv <= 64 * 4) return {1, nv <= 64 ? 1 : nv <= 128 ? 2 : nv <= 192 ? 3 : 4};
-  if (nv <= 256 * 8) return {4, nv <= 512 ? 2 : nv <= 1024 ? 4 : 8};
-  return {4, 0};
+  if (nv <= 8) return {8, 1};
+  if (nv <= 16) return {16, 1};
+  if (nv <= 32) return {32, 1};
+  if (nv <= 64) return {64, 1};
+  if (nv <= 64 * (bwd ? 3 : 4) && (R + 3) / 4 >= 256) return {64, nv <= 128 ? 2 : nv <= 192 ? 3 : 4};
+  if (nv <= 256) return {256, 1};
+  if (nv <= 512) return {256, 2};
+  if (nv <= 1024) return {256, 4};
+  if (nv <= 2048) return {512, 4};
+  return {512, 0};
 }
+static int ln_rows_per_block(const LnForm& f) { return f.lanes <= 256 ? 256 / f.lanes : 1; }
+// blocks of the backward launch = partial rows of the weight gradients: as many as are resident at once.  More start when the first ones end and run
+// their whole share alone: 65536 x 1536 bf16 took 173 us with 768 blocks, 135 with 512
 static int ln_blocks(int R, int C) {
-  const LnForm f = ln_form(C);
-  const int want = f.wpr == 1 ? cdiv(R, 4) : R;
-  return want < LN_MAXB ? want : LN_MAXB;
+  const LnForm f = ln_form(R, C, true);
+  const int want = cdiv(R, ln_rows_per_block(f)), most = f.lanes == 512 ? 256 : f.nv == 1 ? 1024 : 512;
+  return want < most ? want : most;
 }
 size_t k_layernorm_workspace_bytes(int R, int C) { return R > 0 && C > 0 ? (size_t)ln_blocks(R, C) * 2 * C * sizeof(float) : 0; }
 
-#define LN_FORMS(X)                                                                                           \
-  switch (f.wpr * 16 + f.nv) {                                                                                \
-    case 17: X(1, 1); break;                                                                                  \
-    case 18: X(1, 2); break;                                                                                  \
-    case 19: X(1, 3); break;                                                                                  \
-    case 20: X(1, 4); break;                                                                                  \
-    case 66: X(4, 2); break;                                                                                  \
-    case 68: X(4, 4); break;                                                                                  \
-    case 72: X(4, 8); break;                                                                                  \
-    default: X(4, 0); break;                                                                                  \
+#define LN_FORMS(X, X4, X0)                                                                                       \
+  switch (f.lanes * 8 + f.nv) {                                                                               \
+    case 8 * 8 + 1: X(8, 1); break;                                                                           \
+    case 16 * 8 + 1: X(16, 1); break;                                                                         \
+    case 32 * 8 + 1: X(32, 1); break;                                                                         \
+    case 64 * 8 + 1: X(64, 1); break;                                                                         \
+    case 64 * 8 + 2: X(64, 2); break;                                                                         \
+    case 64 * 8 + 3: X(64, 3); break;                                                                         \
+    case 64 * 8 + 4: X4; break;                                                                               \
+    case 256 * 8 + 1: X(256, 1); break;                                                                       \
+    case 256 * 8 + 2: X(256, 2); break;                                                                       \
+    case 256 * 8 + 4: X(256, 4); break;                                                                       \
+    case 512 * 8 + 4: X(512, 4); break;                                                                       \
+    default: X0; break;                                                                                       \
   }
 
 template <typename T> static void ln_fwd(const void* x, long long ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, long long ldy,
                                          float* mean, float* rstd, hipStream_t st) {
-  const LnForm f = ln_form(C);
-  const int grid = f.wpr == 1 ? cdiv(R, 4) : R;
-#define LN_X(W, V) hipLaunchKernelGGL((layernorm_fwd_kernel<T, W, V>), dim3(grid), dim3(LN_T), 0, st, (const T*)x, ldx, gamma, beta, R, C, eps, (T*)y, ldy, mean, rstd)
-  LN_FORMS(LN_X)
+  const LnForm f = ln_form(R, C, false);
+  const int grid = cdiv(R, ln_rows_per_block(f));
+#define LN_X(W, V) hipLaunchKernelGGL((layernorm_fwd_kernel<T, W, V>), dim3(grid), dim3(LN_THREADS(W)), 0, st, (const T*)x, ldx, gamma, beta, R, C, eps, (T*)y, ldy, mean, rstd)
+  LN_FORMS(LN_X, LN_X(64, 4), LN_X(512, 0))
 #undef LN_X
 }
 template <typename T, bool WG> static void ln_bwd(const void* x, long long ldx, const float* gamma, const float* mean, const float* rstd, const void* dy, long long lddy,
                                                   const void* add, long long ldadd, int R, int C, void* dx, long long lddx, float* ws, hipStream_t st) {
-  const LnForm f = ln_form(C);
+  const LnForm f = ln_form(R, C, true);
   const int grid = ln_blocks(R, C);
-#define LN_X(W, V)                                                                                                                                       \
-  hipLaunchKernelGGL((layernorm_bwd_kernel<T, W, V, WG>), dim3(grid), dim3(LN_T), 0, st, (const T*)x, ldx, gamma, mean, rstd, (const T*)dy, lddy, (const T*)add, \
-                     ldadd, R, C, (T*)dx, lddx, ws)
-  LN_FORMS(LN_X)
+#define LN_ARGS(TH) dim3(grid), dim3(TH), 0, st, (const T*)x, ldx, gamma, mean, rstd, (const T*)dy, lddy, (const T*)add, ldadd, R, C, (T*)dx, lddx, ws
+#define LN_X(W, V) hipLaunchKernelGGL((layernorm_bwd_kernel<T, W, V, WG>), LN_ARGS(LN_THREADS(W)))
+#define LN_LONG hipLaunchKernelGGL((layernorm_bwd_long_kernel<T, WG>), LN_ARGS(512))
+  LN_FORMS(LN_X, break, LN_LONG)          // (64, 4) is a forward form only
 #undef LN_X
+#undef LN_LONG
+#undef LN_ARGS
 }
 
 int k_layernorm_fwd(const void* x, long long ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, long long ldy, float* mean, float* rstd,

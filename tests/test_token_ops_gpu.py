@@ -36,7 +36,7 @@ def offset_copy(t, off):
 
 
 # ------------------------------------------------------------------------------------------------ layer norm
-LN = [(1, 1), (3, 2), (5, 7), (2, 8), (9, 63), (4, 65), (17, 512), (33, 520), (128, 2048), (6, 1000), (1030, 96), (4100, 40), (5, 2049), (3, 4099), (7, 8192), (2, 16384),
+LN = [(1, 1), (70, 64), (1100, 71), (37, 130), (2100, 128), (50, 250), (1500, 300), (1, 7000), (3, 2), (5, 7), (2, 8), (9, 63), (4, 65), (17, 512), (33, 520), (128, 2048), (6, 1000), (1030, 96), (4100, 40), (5, 2049), (3, 4099), (7, 8192), (2, 16384),
       (3, 16391), (2, 40000)]
 
 

@@ -56,6 +56,14 @@ __device__ __forceinline__ bool mh_where(const MhaParams& P, int& unit, int& til
   unit = x ? u * 8 + (blockIdx.x & 7) : u;
   return unit < P.units;
 }
+// Ranges of the summed axis (at most `most`).  256 workgroups give every CU one, and a split costs an fp32 partial written, read and joined: full batches are
+// split only below that, into ~512.  With lengths the work per workgroup varies by as much as they do, and the longest decides: ~1024.
+static inline int mh_splits(long long wgs, long long most, bool lengths) {
+  if (wgs <= 0 || (!lengths && wgs >= 256)) return 1;
+  long long s = (lengths ? 1024 : 512) / wgs;
+  if (s > most) s = most;
+  return s < 1 ? 1 : (int)s;
+}
 static inline long long mh_grid(const MhaParams& P) {
   return (long long)(mh_by_xcd(P.units) ? (P.units + 7) / 8 * 8 : P.units) * P.tiles * P.splits;
 }

@@ -13,6 +13,8 @@
 #include "kernels.h"
 #include "mha.h"
 
+#define MH_SHORT 256
+
 // 16 lanes a row, 8 channels a lane (D <= 128)
 template <typename T> __global__ void __launch_bounds__(256) mha_delta_kernel(const MhaParams P) {
   const long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4), n = (long long)P.B * P.Hq * P.Tq;
@@ -90,6 +92,43 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
 
   MhStage<T, NP, KT, DP, WH> sk, sv;
   sk.init(P.kt, P.D); sv.init(P.vt, P.D);
+  // bf16: delta from the ROUNDED o is off by 2^-9 sum |dO||O|, which rows over few keys (large |O|) feel as much as all other roundings together.  Tiles that see
+  // at most MH_SHORT keys take it exactly, delta = sum_j p dP, in a sweep of its own over those keys, and leave it for the dK / dV kernel.
+  if (NP == 1 && nk > 0 && nk <= MH_SHORT) {
+    float acc = 0.f;
+    for (int it = 0; it < ntiles; ++it) {
+      __syncthreads();
+      sk.load(kbase, P.kt, it * KT, 0, lk, mh_sm);
+      sv.load(vbase, P.vt, it * KT, 0, lk, mh_sm + TE);
+      sk.store(mh_sm); sv.store(mh_sm + TE);
+      mh_arrive<decltype(sk)::DMA>();
+      __syncthreads();
+#pragma unroll 1
+      for (int kb = 0; kb < KB; ++kb) {
+        mh_f32x16 S, E;
+        mh_zero(S); mh_zero(E);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          mh_bf16x8 A[NP];
+          mh_frag_rows<NP, KT, DP>(mh_sm, kb * 32, ks, li, h, A);
+          mh_mma<NP>(A, Q[ks], S);
+          mh_frag_rows<NP, KT, DP>(mh_sm + TE, kb * 32, ks, li, h, A);
+          mh_mma<NP>(A, G[ks], E);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], P.sc2, -lse2)) * E[r];
+          acc += it * KT + kb * 32 + 4 * h + (r & 3) + 8 * (r >> 2) < kmax ? x : 0.f;
+        }
+      }
+    }
+    acc += __shfl_xor(acc, 32);
+    if (ok) {
+      del = acc;
+      if (split == 0 && h == 0) P.delta[((long long)b * P.Hq + hq) * P.Tq + tq] = acc;
+    }
+    __syncthreads();
+  }
   if (tb < te) {
     sk.load(kbase, P.kt, tb * KT, 0, lk, mh_sm);
     sv.load(vbase, P.vt, tb * KT, 0, lk, mh_sm + TE);
@@ -320,48 +359,51 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
   }
 }
 
-// out[b][t][h][d] = sum over splits of part[s][(b, h, t)][d], in order; `step`: floats between two ranges
-template <typename T>
+// out[b][t][h][d ..] = sum over splits of part[s][(b, h, t)][d ..], in order; `step`: floats between two ranges.  V channels a thread.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) mha_bwd_join_kernel(const float* __restrict__ part, long long step, int splits, T* out, long long sb, long long stt, long long sh,
-                                                           int H, int Tn, int D, long long n) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float s = 0.f;
-  for (int k = 0; k < splits; ++k) s += part[k * step + i];
-  const int d = (int)(i % D);
-  const long long row = i / D;
-  const int tok = (int)(row % Tn), hh = (int)(row / Tn % H), b = (int)(row / Tn / H);
-  TkVec<T>::store(out + b * sb + (long long)tok * stt + (long long)hh * sh + d, s);
+                                                           int H, int Tn, int D, long long rows) {
+  const int dv = D / V;
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x, row = e / dv;
+  if (row >= rows) return;
+  const int c = (int)(e - row * dv) * V, tok = (int)(row % Tn), hh = (int)(row / Tn % H), b = (int)(row / Tn / H);
+  float s[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[j] = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < splits; ++k) {
+    float v[V];
+    __builtin_memcpy(v, part + k * step + row * D + c, 4 * V);
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] += v[j];
+  }
+  T* o = out + b * sb + (long long)tok * stt + (long long)hh * sh;
+  if constexpr (V == 4) mh_store4<T, true>(o, c, D, s[0], s[1], s[2], s[3]);
+  else TkVec<T>::store(o + c, s[0]);
 }
 
 // ---- host
-// Ranges of the summed axis when the tiles alone give fewer than two workgroups a CU; at least 4 tiles of the summed axis a range.
-static int mh_bwd_splits(long long wgs, long long axis_tiles) {
-  if (wgs <= 0) return 1;
-  long long s = (512 + wgs - 1) / wgs;
-  if (s > axis_tiles / 4) s = axis_tiles / 4;
-  return s < 1 ? 1 : (int)s;
-}
 struct MhaBwdPlan { int dq_tiles, dq_splits, dkv_tiles, dkv_splits; size_t delta_floats, dq_floats, dkv_floats; };
-static MhaBwdPlan mh_bwd_plan(const MhaParams& P) {
+static MhaBwdPlan mh_bwd_plan(const MhaParams& P, bool lengths) {
   MhaBwdPlan L = {};
   L.delta_floats = ((size_t)P.B * P.Hq * P.Tq + 3) / 4 * 4;
   if (P.Tq > 0) {
     L.dq_tiles = cdiv(P.Tq, 128);
-    L.dq_splits = mh_bwd_splits((long long)L.dq_tiles * P.B * P.Hq, cdiv(P.Tk, 64));
+    L.dq_splits = mh_splits((long long)L.dq_tiles * P.B * P.Hq, P.Tk / 256, lengths);
     if (L.dq_splits > 1) L.dq_floats = (size_t)L.dq_splits * P.B * P.Hq * P.Tq * P.D;
   }
   if (P.Tk > 0) {
     L.dkv_tiles = cdiv(P.Tk, 128);
-    L.dkv_splits = mh_bwd_splits((long long)L.dkv_tiles * P.B * P.Hkv, (long long)cdiv(P.Tq, 32) * P.G);
+    L.dkv_splits = mh_splits((long long)L.dkv_tiles * P.B * P.Hkv, (long long)P.Tq * P.G / 128, lengths);
     if (L.dkv_splits > 1) L.dkv_floats = (size_t)L.dkv_splits * 2 * P.B * P.Hkv * P.Tk * P.D;
   }
   return L;
 }
-size_t k_mha_bwd_workspace_bytes(const MhaParams& P) {
-  const MhaBwdPlan L = mh_bwd_plan(P);                                         // dQ and dK / dV partials share their space: the kernels run one after the other
+// dQ and dK / dV partials share their space: the kernels run one after the other
+static size_t mh_bwd_bytes(const MhaBwdPlan& L) {
   return (L.delta_floats + (L.dq_floats > L.dkv_floats ? L.dq_floats : L.dkv_floats)) * sizeof(float);
 }
+size_t k_mha_bwd_workspace_bytes(const MhaParams& P) { return mh_bwd_bytes(mh_bwd_plan(P, true)); }      // (a call with lengths splits into no fewer ranges)
 
 template <typename T, int DP, int KT, int OCC, bool WH = true> static void mh_dq_go(const MhaParams& P, hipStream_t st) {
   constexpr int lds = 4 * MhTile<MhNP<T>::NP, KT, DP>::ELEMS * 2;
@@ -378,14 +420,15 @@ template <typename T, int DP, int QT, int OCC, bool WH = true, bool KL = false> 
 template <typename T> static void mh_bwd_join(const float* part, long long step, int splits, void* out, long long sb, long long stt, long long sh, int H, int Tn, int D,
                                               long long rows, hipStream_t st) {
   const long long n = rows * D;
-  hipLaunchKernelGGL((mha_bwd_join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, step, splits, (T*)out, sb, stt, sh, H, Tn, D, n);
+  if (D % 4 == 0) hipLaunchKernelGGL((mha_bwd_join_kernel<T, 4>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, part, step, splits, (T*)out, sb, stt, sh, H, Tn, D, rows);
+  else hipLaunchKernelGGL((mha_bwd_join_kernel<T, 1>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, step, splits, (T*)out, sb, stt, sh, H, Tn, D, rows);
 }
 
 int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStream_t st) {
   MhaParams P = P0;
   const bool bf = dtype == PDAE_DT_BF16;
-  const MhaBwdPlan L = mh_bwd_plan(P);
-  const size_t need = k_mha_bwd_workspace_bytes(P);
+  const MhaBwdPlan L = mh_bwd_plan(P, P.q_len || P.k_len);
+  const size_t need = mh_bwd_bytes(L);
   if (P.B == 0 || (P.Tq == 0 && P.Tk == 0)) return PDAE_OK;
   PDAE_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "mha_bwd: needs %zu bytes of workspace (got %zu)", need, ws ? ws_bytes : (size_t)0);
   P.delta = (float*)ws;

@@ -195,57 +195,64 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
   }
 }
 
-// Adds the key ranges of a split forward: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  One wave per row.
-template <typename T>
+// Adds the key ranges of a split forward: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  One thread per four channels of a row (V = 1: one channel, D % 4).
+template <typename T, int V>
 __global__ void __launch_bounds__(256) mha_join_kernel(const MhaParams P) {
-  const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), n = (long long)P.units * P.R;
+  const int dv = P.D / V;
+  const long long n = (long long)P.units * P.R, e = (long long)blockIdx.x * 256 + threadIdx.x, i = e / dv;
   if (i >= n) return;
-  const int lane = threadIdx.x & 63, unit = (int)(i / P.R), r = (int)(i % P.R), b = unit / P.HP, hq = unit % P.HP * P.GP + r % P.GP, tq = r / P.GP;
+  const int c = (int)(e - i * dv) * V, unit = (int)(i / P.R), r = (int)(i % P.R), b = unit / P.HP, hq = unit % P.HP * P.GP + r % P.GP, tq = r / P.GP;
   const float* ml = P.part + (long long)P.splits * n * P.D;
   float M = -MH_INF;
-  for (int s = 0; s < P.splits; ++s) { const float* e = ml + (s * n + i) * 2; if (e[1] != 0.f) M = fmaxf(M, e[0]); }
-  const float Ms = M == -MH_INF ? 0.f : M;
-  float L = 0.f, o0 = 0.f, o1 = 0.f;
-  const int c = lane * 2;
   for (int s = 0; s < P.splits; ++s) {
-    const float* e = ml + (s * n + i) * 2;
-    const float ls = e[1];
-    if (ls == 0.f) continue;                                                   // an empty range wrote no O
-    const float w = __builtin_amdgcn_exp2f(e[0] - Ms);
-    const float* po = P.part + (s * n + i) * P.D;
-    L += w * ls;
-    if (c < P.D) o0 += w * po[c];
-    if (c + 1 < P.D) o1 += w * po[c + 1];
+    const tk_f32x2 x = *reinterpret_cast<const tk_f32x2*>(ml + (s * n + i) * 2);
+    if (x[1] != 0.f) M = fmaxf(M, x[0]);
+  }
+  const float Ms = M == -MH_INF ? 0.f : M;
+  float L = 0.f, o[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) o[j] = 0.f;
+  for (int s = 0; s < P.splits; ++s) {
+    const tk_f32x2 x = *reinterpret_cast<const tk_f32x2*>(ml + (s * n + i) * 2);
+    if (x[1] == 0.f) continue;                                                 // an empty range wrote no O
+    const float w = __builtin_amdgcn_exp2f(x[0] - Ms);
+    float v[V];
+    __builtin_memcpy(v, P.part + (s * n + i) * P.D + c, 4 * V);
+    L += w * x[1];
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] += w * v[j];
   }
   const float inv = L != 0.f ? 1.0f / L : 0.f;
   T* orow = (T*)P.out + b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh;
-  if (c < P.D) TkVec<T>::store(orow + c, L != 0.f ? o0 * inv : 0.f);
-  if (c + 1 < P.D) TkVec<T>::store(orow + c + 1, L != 0.f ? o1 * inv : 0.f);
-  if (P.lse && lane == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * MH_LN2 : -MH_INF;
+  if constexpr (V == 4) mh_store4<T, true>(orow, c, P.D, L != 0.f ? o[0] * inv : 0.f, L != 0.f ? o[1] * inv : 0.f, L != 0.f ? o[2] * inv : 0.f, L != 0.f ? o[3] * inv : 0.f);
+  else TkVec<T>::store(orow + c, L != 0.f ? o[0] * inv : 0.f);
+  if (P.lse && c == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * MH_LN2 : -MH_INF;
+}
+template <typename T> static void mh_join(const MhaParams& P, hipStream_t st) {
+  const long long n = (long long)P.units * P.R * P.D;
+  if (P.D % 4 == 0) hipLaunchKernelGGL((mha_join_kernel<T, 4>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, P);
+  else hipLaunchKernelGGL((mha_join_kernel<T, 1>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, P);
 }
 
 // ---- host: row packing, key ranges
 static int mh_qb(int dtype, int R, int D) { return dtype == PDAE_DT_BF16 && R > 128 && D <= 64 && D % 8 == 0 ? 2 : 1; }
 // Rows of a tile: with few query tokens the G heads that share a key head become rows of one tile, so its keys are read once for all of them.
-// Then, when the tiles alone do not give every CU two workgroups, the keys are split into ranges of at least 256.
-static void mh_fwd_plan(MhaParams& P, int dtype) {
+// Then, where the tiles do not fill the chip, the keys are split into ranges of at least 256.
+static void mh_fwd_plan(MhaParams& P, int dtype, bool lengths) {
   P.GP = (long long)P.Tq * P.G <= 128 ? P.G : 1;
   P.HP = P.Hq / P.GP;
   P.R = P.Tq * P.GP;
   P.units = P.B * P.HP;
   P.tiles = cdiv(P.R, 128 * mh_qb(dtype, P.R, P.D));
-  const long long wgs = (long long)P.units * P.tiles;
-  long long s = (512 + wgs - 1) / wgs;
-  const long long most = P.Tk / 256;
-  if (s > most) s = most;
-  P.splits = s < 1 ? 1 : (int)s;
+  P.splits = mh_splits((long long)P.units * P.tiles, P.Tk / 256, lengths);
 }
 static size_t mh_fwd_part_floats(const MhaParams& P) { return P.splits > 1 ? (size_t)P.splits * P.units * P.R * (P.D + 2) : 0; }
 
+// (sized for a call with lengths, which splits into no fewer ranges)
 size_t k_mha_fwd_workspace_bytes(const MhaParams& P0, int dtype) {
   MhaParams P = P0;
   if (P.B <= 0 || P.Tq <= 0) return 0;
-  mh_fwd_plan(P, dtype);
+  mh_fwd_plan(P, dtype, true);
   return mh_fwd_part_floats(P) * sizeof(float);
 }
 
@@ -260,7 +267,7 @@ template <typename T, int DP, int QB, int KT, int OCC, bool WH = true> static vo
 int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStream_t st) {
   MhaParams P = P0;
   if (P.B == 0 || P.Tq == 0) return PDAE_OK;
-  mh_fwd_plan(P, dtype);
+  mh_fwd_plan(P, dtype, P.q_len || P.k_len);
   const size_t need = mh_fwd_part_floats(P) * sizeof(float);
   PDAE_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "mha_fwd: needs %zu bytes of workspace (got %zu)", need, ws ? ws_bytes : (size_t)0);
   PDAE_CHECK_ARG(mh_grid(P) < (1ll << 31) && (long long)P.units * P.R < (1ll << 31), "mha_fwd: too many query rows for one launch");
@@ -281,9 +288,9 @@ int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   }
   if (int e = pdae_launch_status("mha_fwd")) return e;
   if (P.splits > 1) {
-    const long long n = (long long)P.units * P.R;
-    if (dtype == PDAE_DT_BF16) hipLaunchKernelGGL((mha_join_kernel<tk_bf16>), dim3(cdiv(n, 4)), dim3(256), 0, st, P);
-    else hipLaunchKernelGGL((mha_join_kernel<float>), dim3(cdiv(n, 4)), dim3(256), 0, st, P);
+    PDAE_CHECK_ARG((long long)P.units * P.R * P.D / 256 < (1ll << 31), "mha_fwd: too many query rows for one launch");
+    if (dtype == PDAE_DT_BF16) mh_join<tk_bf16>(P, st);
+    else mh_join<float>(P, st);
     return pdae_launch_status("mha_join");
   }
   return PDAE_OK;

@@ -177,17 +177,18 @@ template <int DP> __device__ __forceinline__ int mh_swz(int row) {
 template <int NP, int ROWS, int DP> struct MhTile {
   static constexpr int LD = MhLd<DP>::LD, PLANE = ROWS * LD, ELEMS = NP * PLANE;
 };
-// Global -> LDS of ROWS tokens by 256 threads in 16-byte chunks; load() may run while the other buffer is read, the tile is complete after store() + mh_arrive() and a
+// Global -> LDS of ROWS tokens in 16-byte chunks by the block's 256 threads (NT = 64: by one wave for itself); load() may run while the other buffer is read, the tile is complete after store() + mh_arrive() and a
 // barrier.  bf16 with D % 8 == 0 goes straight into LDS (buffer_load .. lds: a wave's 64 chunks land at consecutive addresses, so the LANE picks the
 // channels that belong at its place): no registers hold the tile in flight.  The other formats pass through registers (split, single elements).
-template <typename T, int NP, int ROWS, int DP, bool WH> struct MhStage {
+template <typename T, int NP, int ROWS, int DP, bool WH, int NT = 256> struct MhStage {
   static constexpr bool DMA = NP == 1 && WH;
-  static constexpr int LD = MhLd<DP>::LD, PLANE = ROWS * LD, CPR = DMA ? LD / 8 : DP / 8, CH = ROWS * CPR, N = (CH + 255) / 256, W = sizeof(T) * 2;
+  static constexpr int LD = MhLd<DP>::LD, PLANE = ROWS * LD, CPR = DMA ? LD / 8 : DP / 8, CH = ROWS * CPR, N = (CH + NT - 1) / NT, W = sizeof(T) * 2;
   unsigned r[DMA ? 1 : N][DMA ? 1 : W], off[N];            // chunk in flight; its byte offset from the tile's first row
   int D;
-  __device__ __forceinline__ static int row_of(int l) { return (int)(threadIdx.x + 256 * l) / CPR; }
+  __device__ __forceinline__ static int tid() { return NT == 256 ? (int)threadIdx.x : (int)threadIdx.x & (NT - 1); }
+  __device__ __forceinline__ static int row_of(int l) { return (tid() + NT * l) / CPR; }
   __device__ __forceinline__ static int chunk_of(int l) {
-    const int c = (int)(threadIdx.x + 256 * l) % CPR;
+    const int c = (tid() + NT * l) % CPR;
     return DMA ? c ^ mh_swz<DP>(row_of(l)) : c;
   }
   __device__ __forceinline__ void init(long long stride, int D_) {
@@ -195,23 +196,23 @@ template <typename T, int NP, int ROWS, int DP, bool WH> struct MhStage {
 #pragma unroll
     for (int l = 0; l < N; ++l) {
       const int c = chunk_of(l) * 8;
-      off[l] = (CH % 256 == 0 || (int)threadIdx.x + 256 * l < CH) && c < D ? (unsigned)(row_of(l) * stride + c) * (unsigned)sizeof(T) : MH_OOB;
+      off[l] = (CH % NT == 0 || tid() + NT * l < CH) && c < D ? (unsigned)(row_of(l) * stride + c) * (unsigned)sizeof(T) : MH_OOB;
     }
   }
   // tokens [row0, row0 + ROWS) of base (token stride `stride` elements); those outside [lo, hi) come as zero and are never read
   __device__ __forceinline__ void load(const T* base, long long stride, int row0, int lo, int hi, unsigned short* lds) {
     const T* p = base + (long long)row0 * stride;
     if constexpr (DMA) {
-      static_assert(CH % 256 == 0 || CH < 256, "whole waves");
+      static_assert(CH % NT == 0 || CH < NT, "whole waves");
       const unsigned long long a = (unsigned long long)p;
       const tk_u32x4 s = {(unsigned)a, (unsigned)(a >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
-      const unsigned dst = (unsigned)(size_t)(mh_lds4)(lds) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+      const unsigned dst = (unsigned)(size_t)(mh_lds4)(lds) + (NT == 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024 : 0);
 #pragma unroll
       for (int l = 0; l < N; ++l) {
         const int row = row0 + row_of(l);
         const unsigned o = row >= lo && row < hi ? off[l] : MH_OOB;
-        if (CH % 256 == 0 || __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64 < CH)
-          asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(o), "s"(s), "s"(dst + l * 4096) : "memory", "m0");
+        if (CH % NT == 0 || __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64 < CH)
+          asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(o), "s"(s), "s"(dst + l * (NT * 16)) : "memory", "m0");
       }
     } else {
       const __amdgpu_buffer_rsrc_t s = mh_rsrc(p);
@@ -226,7 +227,7 @@ template <typename T, int NP, int ROWS, int DP, bool WH> struct MhStage {
     if constexpr (!DMA) {
 #pragma unroll
       for (int l = 0; l < N; ++l) {
-        if (CH % 256 != 0 && (int)threadIdx.x + 256 * l >= CH) continue;
+        if (CH % NT != 0 && tid() + NT * l >= CH) continue;
         unsigned short* d = lds + row_of(l) * LD + (chunk_of(l) ^ mh_swz<DP>(row_of(l))) * 8;
         mh_bf16x8 f[NP];
         mh_raw_planes<T, NP>(r[l], f);
@@ -240,6 +241,7 @@ template <typename T, int NP, int ROWS, int DP, bool WH> struct MhStage {
 template <bool DMA> __device__ __forceinline__ void mh_arrive() {
   if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
+template <int LEFT> __device__ __forceinline__ void mh_arrive_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory"); }      // all but the newest LEFT
 // A fragment, tokens on rows: token row0 + l%32 (row0 a multiple of 32), channels ks * 16 + h * 8 ..+7
 template <int NP, int ROWS, int DP> __device__ __forceinline__ void mh_frag_rows(const unsigned short* lds, int row0, int ks, int li, int h, mh_bf16x8 (&f)[NP]) {
   constexpr int LD = MhLd<DP>::LD;

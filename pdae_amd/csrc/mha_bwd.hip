@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(256) mha_bwd_join_kernel(const float* __restri
   float s[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int k = 0; k < splits; ++k) {
     float v[V];
     __builtin_memcpy(v, part + k * step + row * D + c, 4 * V);

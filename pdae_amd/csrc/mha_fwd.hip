@@ -195,6 +195,137 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
   }
 }
 
+// At most 32 rows (a token, or a few, of the heads that share a key head), bf16: every wave works for itself on 32 keys at a time, loaded straight into its own LDS,
+// double buffered, without a barrier; the waves of a block take turns through its key range and are joined in LDS at the end.  In the kernel above the
+// 128-row tile would leave three waves without rows, and the fourth's latency per tile would be the block's.
+template <int DP, int OCC>
+__global__ void __launch_bounds__(256, OCC) mha_token_kernel(const MhaParams P) {
+  constexpr int KS = DP / 16, DB = DP / 32, TE = MhTile<1, 32, DP>::ELEMS, OL = DP + 4;
+  using Stage = MhStage<tk_bf16, 1, 32, DP, true, 64>;
+  static_assert(Stage::DMA && 32 * OL * 4 + 256 <= 8 * TE, "a wave's result fits its own tiles");
+  extern __shared__ __attribute__((aligned(16))) unsigned short mh_sm[];       // per wave: [2 buffers][K tile | V tile], then its O [32][OL], m[32], l[32] (floats)
+  int unit, tile, split;
+  if (!mh_where(P, unit, tile, split)) return;
+  const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), li = lane & 31, h = lane >> 5;
+  const int b = unit / P.HP, hp = unit % P.HP, hk = hp * P.GP / P.G;
+  const int lq = mh_len(P.q_len, b, P.Tq), lk = mh_len(P.k_len, b, P.Tk), off = lk - lq;
+  const tk_bf16* kbase = (const tk_bf16*)P.k + b * P.kb + hk * P.kh;
+  const tk_bf16* vbase = (const tk_bf16*)P.v + b * P.vb + hk * P.vh;
+  const int nk = max(0, lq <= 0 ? 0 : P.causal ? min(lk, min((P.R - 1) / P.GP, lq - 1) + off + 1) : lk), ntiles = (nk + 31) / 32;
+  const int tb = (int)((long long)ntiles * split / P.splits), te = (int)((long long)ntiles * (split + 1) / P.splits);
+  const int tq = li / P.GP, hq = hp * P.GP + li % P.GP;
+  const bool ok = li < P.R && tq < lq;
+  const int kmax = ok ? (P.causal ? min(lk, tq + off + 1) : lk) : lk;
+  mh_bf16x8 Q[KS][1];
+  mh_row_frags<tk_bf16, 1, DP, true>((const tk_bf16*)P.q + b * P.qb + (long long)hp * P.GP * P.qh,
+                                     ok ? (unsigned)(tq * P.qt + (li % P.GP) * P.qh) * 2u : MH_OOB, P.D, h, Q);
+  unsigned short* mine = mh_sm + wv * 4 * TE;
+  mh_f32x16 O[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) mh_zero(O[d]);
+  float m = -MH_INF, ms = 0.f, l = 0.f;
+  Stage sk, sv;
+  sk.init(P.kt, P.D); sv.init(P.vt, P.D);
+  mh_loads_done();
+  int it = tb + wv, buf = 0;
+  if (it < te) { sk.load(kbase, P.kt, it * 32, 0, lk, mine); sv.load(vbase, P.vt, it * 32, 0, lk, mine + TE); }
+  for (; it < te; it += 4, buf ^= 1) {
+    const unsigned short* cur = mine + buf * 2 * TE;
+    if (it + 4 < te) {
+      unsigned short* nxt = mine + (buf ^ 1) * 2 * TE;
+      sk.load(kbase, P.kt, (it + 4) * 32, 0, lk, nxt); sv.load(vbase, P.vt, (it + 4) * 32, 0, lk, nxt + TE);
+      mh_arrive_but<2 * Stage::N>();
+    } else {
+      mh_arrive_but<0>();
+    }
+    mh_f32x16 S;
+    mh_zero(S);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      mh_bf16x8 A[1];
+      mh_frag_rows<1, 32, DP>(cur, 0, ks, li, h, A);
+      mh_mma<1>(A, Q[ks], S);
+    }
+    mh_order<KS, 4, 1, 1>();
+    __builtin_amdgcn_sched_barrier(0);
+    if (__any(it * 32 + 32 > kmax)) mh_mask_keys(S, it * 32 + 4 * h, kmax);
+    float mx = S[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, S[r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32)) * P.sc2;
+    if (__any(m == -MH_INF || !(mx - m <= 30.f))) {                             // the reference only has to be near the maximum (see above)
+      const float mn = fmaxf(m, mx), msn = mn == -MH_INF ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - msn);
+      m = mn; ms = msn; l *= al;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) O[d][r] *= al;
+    }
+    mh_bf16x8 F[2][1];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[s * 8 + j], P.sc2, -ms)); l += e[j]; }
+      mh_planes<1>(e, F[s]);
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        mh_bf16x8 A[1];
+        mh_frag_cols<1, 32, DP>(cur + TE, s * 16, d, lane, A);
+        mh_mma<1>(A, F[s], O[d]);
+      }
+    mh_order<DB * 2, 4, 2, 1>();
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // join of the four waves, in wave order
+  l += __shfl_xor(l, 32);
+  float* po = reinterpret_cast<float*>(mine);
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<tk_f32x4*>(po + li * OL + d * 32 + g * 8 + h * 4) = tk_f32x4{O[d][g * 4], O[d][g * 4 + 1], O[d][g * 4 + 2], O[d][g * 4 + 3]};
+  if (h == 0) { po[32 * OL + li] = ok && l != 0.f ? m : -MH_INF; po[32 * OL + 32 + li] = ok ? l : 0.f; }
+  __syncthreads();
+  const float* all = reinterpret_cast<const float*>(mh_sm);
+  for (int i = t; i < P.R * (DP / 4); i += 256) {
+    const int r = i / (DP / 4), c = i % (DP / 4) * 4;
+    if (c >= P.D) continue;
+    float M = -MH_INF, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, all[w * 2 * TE + 32 * OL + r]);
+    const float Ms = M == -MH_INF ? 0.f : M;
+    tk_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float lw = all[w * 2 * TE + 32 * OL + 32 + r];
+      if (lw == 0.f) continue;                                                  // a wave without keys
+      const float x = __builtin_amdgcn_exp2f(all[w * 2 * TE + 32 * OL + r] - Ms);
+      const tk_f32x4 v = *reinterpret_cast<const tk_f32x4*>(all + w * 2 * TE + r * OL + c);
+      L += x * lw;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += x * v[j];
+    }
+    if (P.splits > 1) {
+      const long long idx = ((long long)split * P.units + unit) * P.R + r;
+      if (L != 0.f) __builtin_memcpy(P.part + idx * P.D + c, &o, 16);
+      if (c == 0) {
+        float* ml = P.part + (long long)P.splits * P.units * P.R * P.D + idx * 2;
+        ml[0] = M; ml[1] = L;
+      }
+      continue;
+    }
+    const float inv = L != 0.f ? 1.0f / L : 0.f;
+    const int tr = r / P.GP, hr = hp * P.GP + r % P.GP;
+    tk_bf16* orow = (tk_bf16*)P.out + b * P.ob + (long long)tr * P.ot + (long long)hr * P.oh;
+    mh_store4<tk_bf16, true>(orow, c, P.D, L != 0.f ? o[0] * inv : 0.f, L != 0.f ? o[1] * inv : 0.f, L != 0.f ? o[2] * inv : 0.f, L != 0.f ? o[3] * inv : 0.f);
+    if (P.lse && c == 0) P.lse[((long long)b * P.Hq + hr) * P.Tq + tr] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * MH_LN2 : -MH_INF;
+  }
+}
+
 // Adds the key ranges of a split forward: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  One thread per four channels of a row (V = 1: one channel, D % 4).
 template <typename T, int V>
 __global__ void __launch_bounds__(256) mha_join_kernel(const MhaParams P) {
@@ -203,24 +334,27 @@ __global__ void __launch_bounds__(256) mha_join_kernel(const MhaParams P) {
   if (i >= n) return;
   const int c = (int)(e - i * dv) * V, unit = (int)(i / P.R), r = (int)(i % P.R), b = unit / P.HP, hq = unit % P.HP * P.GP + r % P.GP, tq = r / P.GP;
   const float* ml = P.part + (long long)P.splits * n * P.D;
+  // loads of eight ranges in flight: one by one, 32 ranges of a single token were 30 us of latency
   float M = -MH_INF;
+#pragma unroll 8
   for (int s = 0; s < P.splits; ++s) {
     const tk_f32x2 x = *reinterpret_cast<const tk_f32x2*>(ml + (s * n + i) * 2);
-    if (x[1] != 0.f) M = fmaxf(M, x[0]);
+    M = fmaxf(M, x[1] != 0.f ? x[0] : -MH_INF);
   }
   const float Ms = M == -MH_INF ? 0.f : M;
   float L = 0.f, o[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) o[j] = 0.f;
+#pragma unroll 8
   for (int s = 0; s < P.splits; ++s) {
     const tk_f32x2 x = *reinterpret_cast<const tk_f32x2*>(ml + (s * n + i) * 2);
-    if (x[1] == 0.f) continue;                                                 // an empty range wrote no O
-    const float w = __builtin_amdgcn_exp2f(x[0] - Ms);
+    const bool any = x[1] != 0.f;                                              // an empty range wrote no O: what lies there is not used
+    const float w = any ? __builtin_amdgcn_exp2f(x[0] - Ms) : 0.f;
     float v[V];
     __builtin_memcpy(v, P.part + (s * n + i) * P.D + c, 4 * V);
     L += w * x[1];
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] += w * v[j];
+    for (int j = 0; j < V; ++j) o[j] += any ? w * v[j] : 0.f;
   }
   const float inv = L != 0.f ? 1.0f / L : 0.f;
   T* orow = (T*)P.out + b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh;
@@ -245,6 +379,12 @@ static void mh_fwd_plan(MhaParams& P, int dtype, bool lengths) {
   P.units = P.B * P.HP;
   P.tiles = cdiv(P.R, 128 * mh_qb(dtype, P.R, P.D));
   P.splits = mh_splits((long long)P.units * P.tiles, P.Tk / 256, lengths);
+}
+static bool mh_token(const MhaParams& P, int dtype) { return dtype == PDAE_DT_BF16 && P.R <= 32 && P.D % 8 == 0; }
+template <int DP, int OCC> static void mh_token_go(const MhaParams& P, hipStream_t st) {
+  constexpr int lds = 16 * MhTile<1, 32, DP>::ELEMS * 2;
+  hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_token_kernel<DP, OCC>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL((mha_token_kernel<DP, OCC>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
 }
 static size_t mh_fwd_part_floats(const MhaParams& P) { return P.splits > 1 ? (size_t)P.splits * P.units * P.R * (P.D + 2) : 0; }
 
@@ -273,7 +413,12 @@ int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   PDAE_CHECK_ARG(mh_grid(P) < (1ll << 31) && (long long)P.units * P.R < (1ll << 31), "mha_fwd: too many query rows for one launch");
   P.part = (float*)ws;
   const int qb = mh_qb(dtype, P.R, P.D);
-  if (dtype == PDAE_DT_BF16) {
+  if (mh_token(P, dtype)) {
+    if (P.D <= 32) mh_token_go<32, 4>(P, st);
+    else if (P.D <= 64) mh_token_go<64, 2>(P, st);
+    else if (P.D <= 96) mh_token_go<96, 1>(P, st);
+    else mh_token_go<128, 1>(P, st);
+  } else if (dtype == PDAE_DT_BF16) {
     if (P.D & 7) mh_fwd_go<tk_bf16, 128, 1, 64, 2, false>(P, st);
     else if (P.D <= 32) { if (qb == 2) mh_fwd_go<tk_bf16, 32, 2, 64, 2>(P, st); else mh_fwd_go<tk_bf16, 32, 1, 64, 2>(P, st); }
     else if (P.D <= 64) { if (qb == 2) mh_fwd_go<tk_bf16, 64, 2, 64, 2>(P, st); else mh_fwd_go<tk_bf16, 64, 1, 64, 2>(P, st); }

@@ -362,7 +362,52 @@ __global__ void __launch_bounds__(256) mha_join_kernel(const MhaParams P) {
   else TkVec<T>::store(orow + c, L != 0.f ? o[0] * inv : 0.f);
   if (P.lse && c == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * MH_LN2 : -MH_INF;
 }
+// The same for few rows in many ranges: a block per row, its G = 256 / lanes groups take every G-th range and are added in group order through LDS (one
+// thread after another through 32 ranges of a single token was 19 us of latency beside 7 us of attention).
+template <typename T>
+__global__ void __launch_bounds__(256) mha_join_row_kernel(const MhaParams P) {
+  __shared__ float wsum[8][129];
+  __shared__ float mls[2][256];
+  const long long n = (long long)P.units * P.R, i = blockIdx.x;
+  const int t = threadIdx.x, lane = t & 31, g = t >> 5, c = lane * 4;                       // D <= 128: 32 lanes of four channels, eight groups
+  const float* ml = P.part + (long long)P.splits * n * P.D;
+  const int S = P.splits;                                                                   // (the host: at most 256)
+  if (t < S) {
+    const tk_f32x2 x = *reinterpret_cast<const tk_f32x2*>(ml + (t * n + i) * 2);
+    mls[0][t] = x[1] != 0.f ? x[0] : -MH_INF; mls[1][t] = x[1];
+  }
+  __syncthreads();
+  float M = -MH_INF;
+  for (int s = 0; s < S; ++s) M = fmaxf(M, mls[0][s]);
+  const float Ms = M == -MH_INF ? 0.f : M;
+  float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = g; s < S; s += 8) {
+    const float l = mls[1][s], w = l != 0.f ? __builtin_amdgcn_exp2f(mls[0][s] - Ms) : 0.f;
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = c + j < P.D ? P.part[(s * n + i) * P.D + c + j] : 0.f;
+    L += w * l;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] += l != 0.f ? w * v[j] : 0.f;                          // an empty range wrote no O
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) wsum[g][c + j] = o[j];
+  if (lane == 0) wsum[g][128] = L;
+  __syncthreads();
+  if (t >= P.D) return;
+  float x = 0.f, l = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) { x += wsum[k][t]; l += wsum[k][128]; }
+  const int unit = (int)(i / P.R), r = (int)(i % P.R), b = unit / P.HP, hq = unit % P.HP * P.GP + r % P.GP, tq = r / P.GP;
+  TkVec<T>::store((T*)P.out + b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh + t, l != 0.f ? x / l : 0.f);
+  if (P.lse && t == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = l != 0.f ? (M + __builtin_amdgcn_logf(l)) * MH_LN2 : -MH_INF;
+}
 template <typename T> static void mh_join(const MhaParams& P, hipStream_t st) {
+  if (P.splits >= 4 && P.splits <= 256 && (long long)P.units * P.R <= 65536) {
+    hipLaunchKernelGGL((mha_join_row_kernel<T>), dim3((unsigned)((long long)P.units * P.R)), dim3(256), 0, st, P);
+    return;
+  }
   const long long n = (long long)P.units * P.R * P.D;
   if (P.D % 4 == 0) hipLaunchKernelGGL((mha_join_kernel<T, 4>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, P);
   else hipLaunchKernelGGL((mha_join_kernel<T, 1>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, P);

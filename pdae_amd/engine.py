@@ -305,6 +305,10 @@ class Builder:
         self.s2_fwd_max = int(os.environ.get("PDAE_S2_FWD_M", "8192"))
         self._dyf = None
         self._ystats = {}         # id(tensor) -> (tensor, partial sums, wave-tiles per image)
+        # PDAE_ATTN_ANY=1: attention at shapes the fused image kernels do not take (T beyond 256 or no multiple of 64, odd head widths up to 128) runs on
+        # pdae_mha_fwd / _bwd, which store no T x T probabilities (a 64 x 64 level at B = 32 keeps 2 GiB of them per head otherwise).  Off by default: the
+        # GEMM + softmax composition such plans were built on rounds in another order.
+        self.any_attn = os.environ.get("PDAE_ATTN_ANY", "0") == "1"
         self.fuse_attn = os.environ.get("PDAE_FUSE_ATTN", "1") != "0"  # QK^T -> softmax -> PV (and its backward) as one kernel (pdae_attn_fwd / _bwd)
         self.group_wprep = os.environ.get("PDAE_GROUP_WPREP", "1") != "0"   # prepared copies of trainable weights: one grouped launch per run (Plan.pre_arr)
         self.frozen_of = frozen_of      # FlatModule owning `params`: enables the persistent prepared-weight cache for its frozen part
@@ -953,8 +957,15 @@ class Builder:
         scale2 = 1.0 / math.sqrt(ch)          # (ch^-1/4)^2 : q and k are each scaled by ch^-1/4 (module.py:451-453)
         o = pl.buf(N, Hh, W, C)
         fused = self.fuse_attn and H.attn_fused_ok(T, C, heads)
-        Pm = lse = None
-        if fused:
+        Pm = lse = mha = None
+        if not fused and self.any_attn and ch <= 128:
+            st = (T * 3 * C, 3 * C, hs)
+            mha = H.Mha(N, T, T, heads, heads, ch, scale=scale2, q_stride=st, k_stride=st, v_stride=st, o_stride=(T * C, C, ch))
+            lse = pl.buf(N * heads, T) if self.save else None
+            p0 = qkv.data_ptr()
+            pl.need_ws(mha.ws_bytes(False))
+            pl.emit(H.op_mha_fwd(mha, p0 + 4 * oq, p0 + 4 * ok, p0 + 4 * ov, o, lse=lse), ws_slot=7, wsb_slot=20)
+        elif fused:
             # QK^T -> softmax -> PV in one launch, probabilities never written (pdae_attn_fwd); only the row log-sum-exp is kept for backward
             lse = pl.buf(N * heads, T) if self.save else None
             pl.emit(H.op_attn_fwd(qkv, N, T, C, heads, new_order, o, lse))
@@ -970,7 +981,7 @@ class Builder:
         if not self.save:
             pl.free(qkv, Pm, o)
         return out, NS(pre=pre, gx=gx, cq=cq, cp=cp, qkv=qkv, Pm=Pm, lse=lse, o=o, N=N, T=T, C=C, heads=heads, ch=ch, offs=(oq, ok, ov, hs), scale2=scale2,
-                       shape=(N, Hh, W, C), new_order=bool(new_order))
+                       shape=(N, Hh, W, C), new_order=bool(new_order), mha=mha)
 
     def attention_bwd(self, a, dout, need_dx=True, dout_amax=None, out_amax=False):
         """Returns (dx, amax of dx or None); dout_amax / out_amax as in resblock_bwd."""
@@ -980,6 +991,12 @@ class Builder:
         self.conv_bwd_params(a.cp, dout, amax=dout_amax)
         d_o = self.conv_dgrad(a.cp, dout, amax=dout_amax)          # [N,H,W,C]
         dqkv = pl.buf(*a.qkv.shape)
+        if a.mha is not None:
+            p0, d0 = a.qkv.data_ptr(), dqkv.data_ptr()
+            pl.need_ws(a.mha.ws_bytes(True))
+            pl.emit(H.op_mha_bwd(a.mha, p0 + 4 * oq, p0 + 4 * ok, p0 + 4 * ov, a.o, a.lse, d_o, d0 + 4 * oq, d0 + 4 * ok, d0 + 4 * ov), ws_slot=11, wsb_slot=20)
+            pl.free(d_o)
+            return self._attention_bwd_tail(a, dout, dqkv, need_dx, out_amax)
         if a.lse is not None:                                      # fused backward: probabilities recomputed from q, k and the saved log-sum-exp
             wsd = pl.buf(N * heads, T)
             pl.emit(H.op_attn_bwd(a.qkv, a.o, a.lse, d_o, N, T, C, heads, a.new_order, dqkv, wsd))

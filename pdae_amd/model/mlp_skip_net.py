@@ -3,11 +3,13 @@
 Planned graph over [B][C] row-major fp32 buffers:
     cond = time_embed(timestep_embedding(t))                                  (:68-69)
     layer i:  u = [h | x] W_i^T + b_i          two GEMMs on the column blocks of W_i, torch.cat (:73-75) never materialised
+              (training, dropout > 0: h is dropped in place behind the activation, pdae_dropout_fwd; the mask is regenerated in the backward)
               e = silu(cond) We_i^T + be_i                                     (:100-101, 125-127)
               h = silu(LayerNorm(u * (1 + e)))   one fused row kernel           (:130-137, pdae_mlp_modln_fwd)
     last layer: plain Linear (:42-47).
 Backward is hand-derived (pdae_mlp_modln_bwd + GEMMs) and bridged to torch autograd like the other front-ends.
 """
+import random
 from collections import OrderedDict
 from types import SimpleNamespace as NS
 
@@ -43,11 +45,9 @@ def mlp_shapes(cfg):
 class MLPSkipNet(PlannedNet):
     def __init__(self, input_channel, model_channel, num_layers, time_emb_channel, use_norm, dropout, device=None, **kwargs):
         super().__init__()
-        if dropout and dropout > 0:
-            raise NotImplementedError("MLPSkipNet dropout > 0 is not built (every shipped *_latent.yml uses dropout 0.0)")
-        assert num_layers >= 2
+        assert num_layers >= 2 and 0.0 <= float(dropout or 0.0) < 1.0
         cfg = dict(input_channel=input_channel, model_channel=model_channel, num_layers=num_layers, time_emb_channel=time_emb_channel,
-                   use_norm=bool(use_norm), dropout=0.0)
+                   use_norm=bool(use_norm), dropout=float(dropout or 0.0))
         object.__setattr__(self, "cfg", cfg)
         self.input_channel = input_channel                      # read by latent_diffusion_sample (gaussian_diffusion.py:404)
         self.time_emb_channel = time_emb_channel
@@ -79,7 +79,9 @@ class MLPSkipNet(PlannedNet):
                 w.copy_(torch.randn(w.shape, device=w.device) * (2.0 / w.shape[1]) ** 0.5)
 
     # ------------------------------------------------------------------ graph
-    def _emit_forward(self, B, x, t):
+    def _emit_forward(self, B, x, t, dropout=0.0):
+        """dropout > 0 (training plans): nn.Dropout behind the activation of every layer but the last (the plain Linear); the mask of layer i is stream i + 1
+        of the (seed, step) that Plan.set_dropout hands to every run."""
         cfg, pl, P = self.cfg, B.p, self.P
         n, ic = cfg["num_layers"], cfg["input_channel"]
         R = x.shape[0]
@@ -109,7 +111,9 @@ class MLPSkipNet(PlannedNet):
                 y = pl.buf(R, out)
                 g = P.get(p + ".norm.weight"); bt = P.get(p + ".norm.bias")
                 pl.emit(H.op_mlp_modln_fwd(u, e, g, bt, R, out, norm, 1, LN_EPS, y, mean, rstd))
-                L.e, L.le, L.mean, L.rstd, L.y, L.norm = e, le, mean, rstd, y, norm
+                L.e, L.le, L.mean, L.rstd, L.y, L.norm, L.drop = e, le, mean, rstd, y, norm, float(dropout)
+                if dropout > 0:
+                    pl.drop_ops.append((pl.emit(H.op_dropout_fwd(y, None, R * out, dropout, y, layer=i + 1)), 2, 3))
                 if not B.save:
                     pl.free(u, e, mean, rstd)
                     if i >= 1:
@@ -137,6 +141,8 @@ class MLPSkipNet(PlannedNet):
             if L.last:
                 du = dy
             else:
+                if L.drop > 0:
+                    pl.drop_ops.append((pl.emit(H.op_dropout_bwd(dy, R * L.out, L.drop, dy, layer=L.i + 1)), 2, 3))
                 du, de = pl.buf(R, L.out), pl.buf(R, L.out)
                 tg = pl.buf(R, L.out) if L.norm else None
                 tb = pl.buf(R, L.out) if L.norm else None
@@ -180,7 +186,8 @@ class MLPSkipNet(PlannedNet):
         return dx
 
     def plan(self, R, train):
-        key = (R, bool(train))
+        drop = self.cfg["dropout"] if train and self.training else 0.0       # fixed at plan-build time: part of the key
+        key = (R, bool(train), drop > 0)
         pl = self._plans.get(key)
         if pl is not None:
             return pl
@@ -188,7 +195,7 @@ class MLPSkipNet(PlannedNet):
         x = p.buf(R, self.cfg["input_channel"])
         t = p.buf(R, dtype=torch.int64)
         B = Builder(p, self.P, self.grads() if train else None, save=bool(train), acc_grads=bool(train))
-        fx = self._emit_forward(B, x, t)
+        fx = self._emit_forward(B, x, t, dropout=drop)
         p.n_fwd = len(p.recs)
         p.d_out = p.dx = None
         if train:
@@ -208,6 +215,8 @@ class MLPSkipNet(PlannedNet):
         def run_fwd(*_):
             p.x.copy_(x)
             p.t.copy_(t)
+            if p.drop_ops:
+                p.set_dropout(random.getrandbits(31), 0)
             p.run(0, p.n_fwd)
             return (p.out.clone(),)
 

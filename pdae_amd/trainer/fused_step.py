@@ -490,7 +490,7 @@ class FusedLatentStep(_FusedStep):
         B = Builder(p, net.P, net.grads(), save=True, acc_grads=self.num_iterations > 1, math=math)
         z_t = p.buf(batch, ic)
         p.emit(H.op_q_sample(self.z0, self.noise, self.t, lcfg["sqrt_alphas_cumprod"], lcfg["sqrt_one_minus_alphas_cumprod"], batch, ic, z_t))
-        fx = net._emit_forward(B, z_t, self.t)
+        fx = net._emit_forward(B, z_t, self.t, dropout=net.cfg["dropout"])
         d_out = p.buf(batch, ic)
         p.emit(H.op_loss(self.noise, fx.out, None, None, None, None, batch, ic, self.loss, None, deps=d_out, l1=1,
                          scale=1.0 / self.num_iterations), ws_slot=9)

@@ -133,3 +133,31 @@ def test_restatements_agree_with_autograd():
         assert float((ln[n][0] - t.detach()).abs().max()) < 1e-12
     keep = R.keep_mask(1 << 16, 0.1, 5, 6)
     assert abs(float(keep.double().mean()) - 0.9) < 6 * math.sqrt(0.09 / (1 << 16))
+
+
+def test_tensor_functions_have_no_cpu_fallback():
+    from pdae_amd import tokens
+    from pdae_amd.hip import PdaeError
+    x = torch.zeros(2, 3, 1, 8)
+    for call in (lambda: tokens.layer_norm(x), lambda: tokens.dropout(x, 0.1, 0), lambda: tokens.attention(x, x, x)):
+        with pytest.raises(PdaeError, match="ROCm device"):
+            call()
+
+
+def test_latent_denoiser_plans_dropout():
+    """MLPSkipNet's training plan drops behind every layer but the last, once per direction, with a stream per layer; evaluation and sampling plans do not."""
+    from pdae_amd import hip as H
+    from pdae_amd.model.mlp_skip_net import MLPSkipNet
+    net = MLPSkipNet(input_channel=16, model_channel=32, num_layers=4, time_emb_channel=8, use_norm=True, dropout=0.1, device="cpu")
+    kinds = lambda p: [(r.kind, r.i[4], round(r.f[0], 6)) for r in p.recs if r.kind in (H.OP_DROPOUT_FWD, H.OP_DROPOUT_BWD)]
+    net.train()
+    p = net.plan(4, True)
+    assert kinds(p) == [(H.OP_DROPOUT_FWD, i, 0.1) for i in (1, 2, 3)] + [(H.OP_DROPOUT_BWD, i, 0.1) for i in (3, 2, 1)]
+    p.set_dropout(12345, 6)
+    assert all(p.arr[k].i[2] == 12345 and p.arr[k].i[3] == 6 for k, _, _ in p.drop_ops) and len(p.drop_ops) == 6
+    assert not kinds(net.plan(4, False))
+    net.eval()
+    assert not kinds(net.plan(4, True))
+    for bad in (1.0, -0.1):
+        with pytest.raises(AssertionError):
+            MLPSkipNet(input_channel=16, model_channel=32, num_layers=3, time_emb_channel=8, use_norm=True, dropout=bad, device="cpu")

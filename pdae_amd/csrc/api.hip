@@ -839,7 +839,7 @@ extern "C" size_t pdae_mha_workspace_bytes(const pdae_mha_desc* d, int backward)
   if (mha_params(d, 0, P)) return 0;
   const size_t f = k_mha_fwd_workspace_bytes(P, d->dtype);
   if (!backward) return f;
-  const size_t b = k_mha_bwd_workspace_bytes(P);
+  const size_t b = k_mha_bwd_workspace_bytes(P, d->dtype);
   return b > f ? b : f;                          // one buffer serves the forward and the backward that follows it
 }
 extern "C" int pdae_mha_fwd(const pdae_mha_desc* d, const void* q, const void* k, const void* v, const int32_t* q_len, const int32_t* k_len, void* o, float* lse, void* ws,

@@ -79,7 +79,7 @@ int k_layernorm_bwd(const void* x, long long ldx, const float* gamma, const floa
                     hipStream_t st);
 struct MhaParams;
 size_t k_mha_fwd_workspace_bytes(const MhaParams& P, int dtype);
-size_t k_mha_bwd_workspace_bytes(const MhaParams& P);
+size_t k_mha_bwd_workspace_bytes(const MhaParams& P, int dtype);
 int k_mha_fwd(const MhaParams& P, int dtype, void* ws, size_t ws_bytes, hipStream_t st);
 int k_mha_bwd(const MhaParams& P, int dtype, void* ws, size_t ws_bytes, hipStream_t st);
 

@@ -56,13 +56,14 @@ __device__ __forceinline__ bool mh_where(const MhaParams& P, int& unit, int& til
   unit = x ? u * 8 + (blockIdx.x & 7) : u;
   return unit < P.units;
 }
-// Ranges of the summed axis (at most `most`).  256 workgroups give every CU one, and a split costs an fp32 partial written, read and joined: full batches are
-// split only below that, into ~512.  With lengths the work per workgroup varies by as much as they do, and the longest decides: ~1024.
-static inline int mh_splits(long long wgs, long long most, bool lengths) {
+// Ranges of the summed axis of `tokens`.  256 workgroups give every CU one, and a split costs an fp32 partial written, read and joined, and a prologue: full batches
+// are split only below that, into ~512 (one fp32 sample of 4 heads, 1568 tokens, forward and backward: 167 us at 208 workgroups, 143 at 312, 146 at 468).  With lengths
+// the work per workgroup varies by as much as they do, and the longest decides: ~1024.  A range is at least two tiles; with lengths (they are cut unevenly) and for
+// single tokens (a wave takes 32 keys a step) twice that: one sample, 8 key heads, 8192 keys: 11.3 us with ranges of 256, 16.1 with 128.
+static inline int mh_splits(long long wgs, long long tokens, int dtype, bool lengths, bool token = false) {
   if (wgs <= 0 || (!lengths && wgs >= 256)) return 1;
-  long long s = (lengths ? 1024 : 512) / wgs;
-  if (s > most) s = most;
-  return s < 1 ? 1 : (int)s;
+  const long long s = (lengths ? 1024 : 512) / wgs, most = tokens / ((dtype == PDAE_DT_BF16 ? 128 : 64) * (lengths || token ? 2 : 1));
+  return (int)(s > most ? most < 1 ? 1 : most : s < 1 ? 1 : s);
 }
 static inline long long mh_grid(const MhaParams& P) {
   return (long long)(mh_by_xcd(P.units) ? (P.units + 7) / 8 * 8 : P.units) * P.tiles * P.splits;
@@ -138,6 +139,13 @@ template <typename T, bool WH> __device__ __forceinline__ void mh_raw8(__amdgpu_
       if constexpr (sizeof(T) == 4) r[j] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(s, o, 0, 0);
       else r[j / 2] |= (unsigned)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(s, o, 0, 0) << (16 * (j & 1));
     }
+  }
+}
+template <typename T> __device__ __forceinline__ void mh_raw_floats(const unsigned (&r)[sizeof(T) * 2], float (&e)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if constexpr (sizeof(T) == 4) e[j] = __uint_as_float(r[j]);
+    else e[j] = __uint_as_float(j & 1 ? r[j / 2] & 0xffff0000u : r[j / 2] << 16);
   }
 }
 template <typename T, int NP> __device__ __forceinline__ void mh_raw_planes(const unsigned (&r)[sizeof(T) * 2], mh_bf16x8 (&f)[NP]) {

@@ -1,9 +1,8 @@
 // Attention backward (mha.h): the probabilities are recomputed from q, k and the saved row log-sum-exp, nothing of size tokens x tokens exists.
 //
-//   delta[q] = sum_d dO[q][d] O[q][d]                         mha_delta_kernel
-//   P = exp(scale q.k - lse),  dP = dO.v,  dS = P (dP - delta)
-//   dV = P^T dO,  dK = scale dS^T Q                           mha_dkv_kernel: a wave owns 32 keys (columns), the queries stream through LDS
-//   dQ = scale dS K                                           mha_dq_kernel:  a wave owns 32 queries (columns), the keys stream through LDS
+//   P = exp(scale q.k - lse),  dP = dO.v,  dS = P (dP - delta),  delta[q] = sum_d dO[q][d] O[q][d] = sum_j P dP
+//   dQ = scale dS K                   mha_dq_kernel:  a wave owns 32 queries (columns), the keys stream through LDS; it also leaves delta for
+//   dV = P^T dO,  dK = scale dS^T Q   mha_dkv_kernel: a wave owns 32 keys (columns), the queries stream through LDS
 //
 // Two kernels recompute S and dP twice (7 products of 2 Tq Tk D instead of 5): dK / dV and dQ then each have ONE writer, so there are no atomics and the
 // results are the same bits every run.  dK / dV of a key head sum over the query heads that share it inside the kernel.
@@ -14,32 +13,6 @@
 #include "mha.h"
 
 #define MH_SHORT 256
-
-// 16 lanes a row, 8 channels a lane (D <= 128)
-template <typename T> __global__ void __launch_bounds__(256) mha_delta_kernel(const MhaParams P) {
-  const long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4), n = (long long)P.B * P.Hq * P.Tq;
-  if (i >= n) return;
-  const int c = (threadIdx.x & 15) * 8, tq = (int)(i % P.Tq), hq = (int)(i / P.Tq % P.Hq), b = (int)(i / P.Tq / P.Hq);
-  const int lq = mh_len(P.q_len, b, P.Tq);
-  float s = 0.f;
-  if (tq < lq && c < P.D) {
-    float x[8], y[8];
-    const long long at = b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh;
-    if (c + 8 <= P.D) { TkVec<T>::load8((const T*)P.o + at + c, x); TkVec<T>::load8((const T*)P.d_o + at + c, y); }
-    else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = c + j < P.D ? TkVec<T>::load((const T*)P.o + at + c + j) : 0.f;
-        y[j] = c + j < P.D ? TkVec<T>::load((const T*)P.d_o + at + c + j) : 0.f;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s += x[j] * y[j];
-  }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if ((threadIdx.x & 15) == 0) P.delta[i] = s;
-}
 
 // accumulators (channels on rows, this lane's token on the column) -> row of a tensor, or fp32 partial row
 template <typename T, int DB, bool WH> __device__ __forceinline__ void mh_put(const mh_f32x16 (&a)[DB], float f, bool keep, T* row, int D, int h) {
@@ -79,12 +52,32 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
                               ok ? (unsigned)((tq - row0) * P.qt) * (unsigned)sizeof(T) : MH_OOB, P.D, h, Q);
   mh_row_frags<T, NP, DP, WH>((const T*)P.d_o + b * P.ob + (long long)row0 * P.ot + (long long)hq * P.oh,
                               ok ? (unsigned)((tq - row0) * P.ot) * (unsigned)sizeof(T) : MH_OOB, P.D, h, G);
-  float lse2 = MH_INF, del = 0.f;
+  const long long row = ((long long)b * P.Hq + hq) * P.Tq + tq;
+  float lse2 = MH_INF;
+  // delta of this lane's query from dO and O: half of the channels here, half 32 lanes away.  (A launch of its own for it read both once more: 35 us of 4 x 16
+  // heads of 128, 4096 tokens.)
+  float del = 0.f;
+  {
+    const __amdgpu_buffer_rsrc_t so = mh_rsrc((const T*)P.o + b * P.ob + (long long)row0 * P.ot + (long long)hq * P.oh);
+    const __amdgpu_buffer_rsrc_t sg = mh_rsrc((const T*)P.d_o + b * P.ob + (long long)row0 * P.ot + (long long)hq * P.oh);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int c = ks * 16 + h * 8;
+      const unsigned at = ok && c < P.D ? (unsigned)((tq - row0) * P.ot + c) * (unsigned)sizeof(T) : MH_OOB;
+      unsigned x[sizeof(T) * 2], y[sizeof(T) * 2];
+      mh_raw8<T, WH>(so, at, P.D - c, x);
+      mh_raw8<T, WH>(sg, at, P.D - c, y);
+      float e[8], f[8];
+      mh_raw_floats<T>(x, e);
+      mh_raw_floats<T>(y, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) del += e[j] * f[j];
+    }
+    del += __shfl_xor(del, 32);
+  }
   if (ok) {
-    const long long i = ((long long)b * P.Hq + hq) * P.Tq + tq;
-    const float e = P.lse[i];
+    const float e = P.lse[row];
     lse2 = e == -MH_INF ? MH_INF : e * MH_LOG2E;
-    del = P.delta[i];
   }
   mh_f32x16 dQ[DB];
 #pragma unroll
@@ -93,7 +86,7 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
   MhStage<T, NP, KT, DP, WH> sk, sv;
   sk.init(P.kt, P.D); sv.init(P.vt, P.D);
   // bf16: delta from the ROUNDED o is off by 2^-9 sum |dO||O|, which rows over few keys (large |O|) feel as much as all other roundings together.  Tiles that see
-  // at most MH_SHORT keys take it exactly, delta = sum_j p dP, in a sweep of its own over those keys, and leave it for the dK / dV kernel.
+  // at most MH_SHORT keys take it exactly, delta = sum_j p dP, in a sweep of its own over those keys, too.
   if (NP == 1 && nk > 0 && nk <= MH_SHORT) {
     float acc = 0.f;
     for (int it = 0; it < ntiles; ++it) {
@@ -123,12 +116,10 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
       }
     }
     acc += __shfl_xor(acc, 32);
-    if (ok) {
-      del = acc;
-      if (split == 0 && h == 0) P.delta[((long long)b * P.Hq + hq) * P.Tq + tq] = acc;
-    }
+    if (ok) del = acc;
     __syncthreads();
   }
+  if (ok && split == 0 && h == 0) P.delta[row] = del;
   if (tb < te) {
     sk.load(kbase, P.kt, tb * KT, 0, lk, mh_sm);
     sv.load(vbase, P.vt, tb * KT, 0, lk, mh_sm + TE);
@@ -190,8 +181,7 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
   }
   if (tq >= P.Tq) return;
   if (P.splits > 1) {
-    float* row = P.part + (((long long)split * P.B * P.Hq + unit) * P.Tq + tq) * P.D;
-    mh_put<float, DB, WH>(dQ, P.scale, ok, row, P.D, h);
+    mh_put<float, DB, WH>(dQ, P.scale, ok, P.part + ((long long)split * P.B * P.Hq * P.Tq + row) * P.D, P.D, h);
   } else {
     mh_put<T, DB, WH>(dQ, P.scale, ok, (T*)P.dq + b * P.qb + (long long)tq * P.qt + (long long)hq * P.qh, P.D, h);
   }
@@ -359,42 +349,46 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
   }
 }
 
-// out[b][t][h][d ..] = sum over splits of part[s][(b, h, t)][d ..], in order; `step`: floats between two ranges.  V channels a thread.
+// out[b][t][h][d ..] = sum over splits of part[s][(b, h, t)][d ..], in order; `step`: floats between two ranges.  V channels a thread.  blockIdx.y: which
+// of two tensors (their partials lie behind one another).
+struct MhaJoinTo { void* p; long long sb, st, sh; };
 template <typename T, int V>
-__global__ void __launch_bounds__(256) mha_bwd_join_kernel(const float* __restrict__ part, long long step, int splits, T* out, long long sb, long long stt, long long sh,
-                                                           int H, int Tn, int D, long long rows) {
+__global__ void __launch_bounds__(256) mha_bwd_join_kernel(const float* __restrict__ part, long long step, int splits, MhaJoinTo to0, MhaJoinTo to1, int H, int Tn, int D,
+                                                           long long rows) {
+  const MhaJoinTo to = blockIdx.y ? to1 : to0;
   const int dv = D / V;
   const long long e = (long long)blockIdx.x * 256 + threadIdx.x, row = e / dv;
   if (row >= rows) return;
   const int c = (int)(e - row * dv) * V, tok = (int)(row % Tn), hh = (int)(row / Tn % H), b = (int)(row / Tn / H);
+  const float* p = part + ((long long)blockIdx.y * rows + row) * D + c;
   float s[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = 0.f;
 #pragma unroll 8
   for (int k = 0; k < splits; ++k) {
     float v[V];
-    __builtin_memcpy(v, part + k * step + row * D + c, 4 * V);
+    __builtin_memcpy(v, p + k * step, 4 * V);
 #pragma unroll
     for (int j = 0; j < V; ++j) s[j] += v[j];
   }
-  T* o = out + b * sb + (long long)tok * stt + (long long)hh * sh;
+  T* o = (T*)to.p + b * to.sb + (long long)tok * to.st + (long long)hh * to.sh;
   if constexpr (V == 4) mh_store4<T, true>(o, c, D, s[0], s[1], s[2], s[3]);
   else TkVec<T>::store(o + c, s[0]);
 }
 
 // ---- host
 struct MhaBwdPlan { int dq_tiles, dq_splits, dkv_tiles, dkv_splits; size_t delta_floats, dq_floats, dkv_floats; };
-static MhaBwdPlan mh_bwd_plan(const MhaParams& P, bool lengths) {
+static MhaBwdPlan mh_bwd_plan(const MhaParams& P, int dtype, bool lengths) {
   MhaBwdPlan L = {};
   L.delta_floats = ((size_t)P.B * P.Hq * P.Tq + 3) / 4 * 4;
   if (P.Tq > 0) {
     L.dq_tiles = cdiv(P.Tq, 128);
-    L.dq_splits = mh_splits((long long)L.dq_tiles * P.B * P.Hq, P.Tk / 256, lengths);
+    L.dq_splits = mh_splits((long long)L.dq_tiles * P.B * P.Hq, P.Tk, dtype, lengths);
     if (L.dq_splits > 1) L.dq_floats = (size_t)L.dq_splits * P.B * P.Hq * P.Tq * P.D;
   }
   if (P.Tk > 0) {
     L.dkv_tiles = cdiv(P.Tk, 128);
-    L.dkv_splits = mh_splits((long long)L.dkv_tiles * P.B * P.Hkv, (long long)P.Tq * P.G / 128, lengths);
+    L.dkv_splits = mh_splits((long long)L.dkv_tiles * P.B * P.Hkv, (long long)P.Tq * P.G, dtype, lengths);
     if (L.dkv_splits > 1) L.dkv_floats = (size_t)L.dkv_splits * 2 * P.B * P.Hkv * P.Tk * P.D;
   }
   return L;
@@ -403,7 +397,10 @@ static MhaBwdPlan mh_bwd_plan(const MhaParams& P, bool lengths) {
 static size_t mh_bwd_bytes(const MhaBwdPlan& L) {
   return (L.delta_floats + (L.dq_floats > L.dkv_floats ? L.dq_floats : L.dkv_floats)) * sizeof(float);
 }
-size_t k_mha_bwd_workspace_bytes(const MhaParams& P) { return mh_bwd_bytes(mh_bwd_plan(P, true)); }      // (a call with lengths splits into no fewer ranges)
+size_t k_mha_bwd_workspace_bytes(const MhaParams& P, int dtype) {               // for calls with and without lengths
+  const size_t n = mh_bwd_bytes(mh_bwd_plan(P, dtype, true)), m = mh_bwd_bytes(mh_bwd_plan(P, dtype, false));
+  return n > m ? n : m;
+}
 
 template <typename T, int DP, int KT, int OCC, bool WH = true> static void mh_dq_go(const MhaParams& P, hipStream_t st) {
   constexpr int lds = 4 * MhTile<MhNP<T>::NP, KT, DP>::ELEMS * 2;
@@ -417,17 +414,21 @@ template <typename T, int DP, int QT, int OCC, bool WH = true, bool KL = false> 
   hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_dkv_kernel<T, DP, QT, OCC, WH, KL>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   hipLaunchKernelGGL((mha_dkv_kernel<T, DP, QT, OCC, WH, KL>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
 }
-template <typename T> static void mh_bwd_join(const float* part, long long step, int splits, void* out, long long sb, long long stt, long long sh, int H, int Tn, int D,
-                                              long long rows, hipStream_t st) {
-  const long long n = rows * D;
-  if (D % 4 == 0) hipLaunchKernelGGL((mha_bwd_join_kernel<T, 4>), dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, part, step, splits, (T*)out, sb, stt, sh, H, Tn, D, rows);
-  else hipLaunchKernelGGL((mha_bwd_join_kernel<T, 1>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, step, splits, (T*)out, sb, stt, sh, H, Tn, D, rows);
+static void mh_bwd_join(bool bf, const MhaParams& P, long long step, MhaJoinTo to0, MhaJoinTo to1, int n, int H, int Tn, long long rows, hipStream_t st) {
+  const dim3 grid((unsigned)((rows * P.D / (P.D % 4 ? 1 : 4) + 255) / 256), n);
+  if (P.D % 4 == 0) {
+    if (bf) hipLaunchKernelGGL((mha_bwd_join_kernel<tk_bf16, 4>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, H, Tn, P.D, rows);
+    else hipLaunchKernelGGL((mha_bwd_join_kernel<float, 4>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, H, Tn, P.D, rows);
+  } else {
+    if (bf) hipLaunchKernelGGL((mha_bwd_join_kernel<tk_bf16, 1>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, H, Tn, P.D, rows);
+    else hipLaunchKernelGGL((mha_bwd_join_kernel<float, 1>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, H, Tn, P.D, rows);
+  }
 }
 
 int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStream_t st) {
   MhaParams P = P0;
   const bool bf = dtype == PDAE_DT_BF16;
-  const MhaBwdPlan L = mh_bwd_plan(P, P.q_len || P.k_len);
+  const MhaBwdPlan L = mh_bwd_plan(P, dtype, P.q_len || P.k_len);
   const size_t need = mh_bwd_bytes(L);
   if (P.B == 0 || (P.Tq == 0 && P.Tk == 0)) return PDAE_OK;
   PDAE_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "mha_bwd: needs %zu bytes of workspace (got %zu)", need, ws ? ws_bytes : (size_t)0);
@@ -436,8 +437,6 @@ int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   const long long nq = (long long)P.B * P.Hq * P.Tq, nk = (long long)P.B * P.Hkv * P.Tk;
   PDAE_CHECK_ARG(nq * P.D / 256 < (1ll << 31) && nk * P.D / 256 < (1ll << 31), "mha_bwd: too many rows for one launch");
   if (P.Tq > 0) {
-    if (bf) hipLaunchKernelGGL((mha_delta_kernel<tk_bf16>), dim3(cdiv(nq, 16)), dim3(256), 0, st, P);
-    else hipLaunchKernelGGL((mha_delta_kernel<float>), dim3(cdiv(nq, 16)), dim3(256), 0, st, P);
     P.units = P.B * P.Hq; P.tiles = L.dq_tiles; P.splits = L.dq_splits;
     PDAE_CHECK_ARG(mh_grid(P) < (1ll << 31), "mha_bwd: too many query tiles for one launch");
     if (bf) {
@@ -455,8 +454,8 @@ int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
     }
     if (int e = pdae_launch_status("mha_dq")) return e;
     if (P.splits > 1) {
-      if (bf) mh_bwd_join<tk_bf16>(P.part, nq * P.D, P.splits, P.dq, P.qb, P.qt, P.qh, P.Hq, P.Tq, P.D, nq, st);
-      else mh_bwd_join<float>(P.part, nq * P.D, P.splits, P.dq, P.qb, P.qt, P.qh, P.Hq, P.Tq, P.D, nq, st);
+      const MhaJoinTo to = {P.dq, P.qb, P.qt, P.qh};
+      mh_bwd_join(bf, P, nq * P.D, to, to, 1, P.Hq, P.Tq, nq, st);
     }
   }
   if (P.Tk > 0) {
@@ -476,16 +475,7 @@ int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
       else mh_dkv_go<float, 128, 32, 1>(P, st);
     }
     if (int e = pdae_launch_status("mha_dkv")) return e;
-    if (P.splits > 1) {
-      const long long step = 2 * nk * P.D;
-      if (bf) {
-        mh_bwd_join<tk_bf16>(P.part, step, P.splits, P.dk, P.kb, P.kt, P.kh, P.Hkv, P.Tk, P.D, nk, st);
-        mh_bwd_join<tk_bf16>(P.part + nk * P.D, step, P.splits, P.dv, P.vb, P.vt, P.vh, P.Hkv, P.Tk, P.D, nk, st);
-      } else {
-        mh_bwd_join<float>(P.part, step, P.splits, P.dk, P.kb, P.kt, P.kh, P.Hkv, P.Tk, P.D, nk, st);
-        mh_bwd_join<float>(P.part + nk * P.D, step, P.splits, P.dv, P.vb, P.vt, P.vh, P.Hkv, P.Tk, P.D, nk, st);
-      }
-    }
+    if (P.splits > 1) mh_bwd_join(bf, P, 2 * nk * P.D, MhaJoinTo{P.dk, P.kb, P.kt, P.kh}, MhaJoinTo{P.dv, P.vb, P.vt, P.vh}, 2, P.Hkv, P.Tk, nk, st);
   }
   return pdae_launch_status("mha_bwd");
 }

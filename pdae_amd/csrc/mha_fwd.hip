@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(256) mha_join_row_kernel(const MhaParams P) {
   if (P.lse && t == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = l != 0.f ? (M + __builtin_amdgcn_logf(l)) * MH_LN2 : -MH_INF;
 }
 template <typename T> static void mh_join(const MhaParams& P, hipStream_t st) {
-  if (P.splits >= 4 && P.splits <= 256 && (long long)P.units * P.R <= 65536) {
+  if (P.splits >= 4 && P.splits <= 256 && (long long)P.units * P.R <= 4096) {
     hipLaunchKernelGGL((mha_join_row_kernel<T>), dim3((unsigned)((long long)P.units * P.R)), dim3(256), 0, st, P);
     return;
   }
@@ -414,18 +414,18 @@ template <typename T> static void mh_join(const MhaParams& P, hipStream_t st) {
 }
 
 // ---- host: row packing, key ranges
+static bool mh_token(const MhaParams& P, int dtype) { return dtype == PDAE_DT_BF16 && P.R <= 32 && P.D % 8 == 0; }
 static int mh_qb(int dtype, int R, int D) { return dtype == PDAE_DT_BF16 && R > 128 && D <= 64 && D % 8 == 0 ? 2 : 1; }
 // Rows of a tile: with few query tokens the G heads that share a key head become rows of one tile, so its keys are read once for all of them.
-// Then, where the tiles do not fill the chip, the keys are split into ranges of at least 256.
+// Then, where the tiles do not fill the chip, the keys are split into ranges.
 static void mh_fwd_plan(MhaParams& P, int dtype, bool lengths) {
   P.GP = (long long)P.Tq * P.G <= 128 ? P.G : 1;
   P.HP = P.Hq / P.GP;
   P.R = P.Tq * P.GP;
   P.units = P.B * P.HP;
   P.tiles = cdiv(P.R, 128 * mh_qb(dtype, P.R, P.D));
-  P.splits = mh_splits((long long)P.units * P.tiles, P.Tk / 256, lengths);
+  P.splits = mh_splits((long long)P.units * P.tiles, P.Tk, dtype, lengths, mh_token(P, dtype));
 }
-static bool mh_token(const MhaParams& P, int dtype) { return dtype == PDAE_DT_BF16 && P.R <= 32 && P.D % 8 == 0; }
 template <int DP, int OCC> static void mh_token_go(const MhaParams& P, hipStream_t st) {
   constexpr int lds = 16 * MhTile<1, 32, DP>::ELEMS * 2;
   hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_token_kernel<DP, OCC>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -433,12 +433,15 @@ template <int DP, int OCC> static void mh_token_go(const MhaParams& P, hipStream
 }
 static size_t mh_fwd_part_floats(const MhaParams& P) { return P.splits > 1 ? (size_t)P.splits * P.units * P.R * (P.D + 2) : 0; }
 
-// (sized for a call with lengths, which splits into no fewer ranges)
+// for calls with and without lengths
 size_t k_mha_fwd_workspace_bytes(const MhaParams& P0, int dtype) {
   MhaParams P = P0;
   if (P.B <= 0 || P.Tq <= 0) return 0;
   mh_fwd_plan(P, dtype, true);
-  return mh_fwd_part_floats(P) * sizeof(float);
+  const size_t n = mh_fwd_part_floats(P);
+  mh_fwd_plan(P, dtype, false);
+  const size_t m = mh_fwd_part_floats(P);
+  return (n > m ? n : m) * sizeof(float);
 }
 
 template <typename T, int DP, int QB, int KT, int OCC, bool WH = true> static void mh_fwd_go(const MhaParams& P, hipStream_t st) {

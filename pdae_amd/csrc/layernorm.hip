@@ -7,10 +7,10 @@
 // The variance is taken from the deviations (two passes over registers), not from E[x^2] - E[x]^2, which loses what a large mean leaves.
 //
 // Weight gradients: every block walks a fixed set of rows and keeps sum dy xh / sum dy of its lanes' own channels in registers; it leaves ONE partial row per
-// block, and a second launch adds the partial rows in a fixed order (no atomics: bit-identical from run to run).
+// block, and a second launch adds the partial rows in a fixed order (no atomics: bit-identical from run to run).  Few rows are latency, not bytes: one launch,
+// in which blocks of their own add up the columns.
 #include "token.h"
 #include "kernels.h"
-
 
 // sum over the L lanes that share a row (L <= 64: neighbouring lanes of a wave; else the whole block of L threads)
 template <int L> __device__ __forceinline__ float ln_sum(float v, float* red) {
@@ -114,10 +114,9 @@ template <typename T> __device__ __forceinline__ float ln_elem(const LnRaw<T>& r
 // forms would take four times the registers, and the row AFTER it could not be in flight meanwhile -- with one row at a time a wave waited for HBM
 // on every row (65536 x 1536 bf16: 239 us, 2.5 TB/s).
 template <typename T, int L, int NV, bool WG>
-__global__ void __launch_bounds__(LN_THREADS(L)) layernorm_bwd_kernel(const T* __restrict__ x, long long ldx, const float* __restrict__ gamma,
-                                                             const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ dy,
-                                                             long long lddy, const T* add, long long ldadd, int R, int C, T* dx, long long lddx,
-                                                             float* __restrict__ part) {
+__device__ __forceinline__ void ln_bwd_rows(const T* __restrict__ x, long long ldx, const float* __restrict__ gamma, const float* __restrict__ mean,
+                                            const float* __restrict__ rstd, const T* __restrict__ dy, long long lddy, const T* add, long long ldadd, int R, int C, T* dx,
+                                            long long lddx, float* __restrict__ part, int blocks) {
   __shared__ float red[16];
   __shared__ float comb[L <= 64 && WG ? 2 * L * 9 : 1];
   constexpr int RPB = LN_THREADS(L) / L;
@@ -135,7 +134,7 @@ __global__ void __launch_bounds__(LN_THREADS(L)) layernorm_bwd_kernel(const T* _
   if (gamma && has) gmt = gamma[te];
   LnRaw<T> qx[2][NV], qd[2][NV];
   float tx[2], td[2], mu[2], rs[2];
-  const long long step = (long long)gridDim.x * RPB;
+  const long long step = (long long)blocks * RPB;
   auto fetch = [&](long long row, LnRaw<T> (&rx)[NV], LnRaw<T> (&rd)[NV], float& ex, float& ed, float& m, float& r) __attribute__((always_inline)) {
     const T* xr = x + row * ldx;
     const T* dr = dy + row * lddy;
@@ -242,6 +241,46 @@ __global__ void __launch_bounds__(LN_THREADS(L)) layernorm_bwd_kernel(const T* _
   }
 }
 
+template <typename T, int L, int NV, bool WG>
+__global__ void __launch_bounds__(LN_THREADS(L)) layernorm_bwd_kernel(const T* __restrict__ x, long long ldx, const float* __restrict__ gamma,
+                                                             const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ dy,
+                                                             long long lddy, const T* add, long long ldadd, int R, int C, T* dx, long long lddx,
+                                                             float* __restrict__ part) {
+  ln_bwd_rows<T, L, NV, WG>(x, ldx, gamma, mean, rstd, dy, lddy, add, ldadd, R, C, dx, lddx, part, gridDim.x);
+}
+// Few rows: one launch.  The first `blocks` blocks take rows as above, the others 32 columns each (8 slices of the rows, added in order) and read x and dy
+// of their columns once more.
+template <typename T, int L, int NV>
+__global__ void __launch_bounds__(256) layernorm_bwd_few_kernel(const T* __restrict__ x, long long ldx, const float* __restrict__ gamma, const float* __restrict__ mean,
+                                                                const float* __restrict__ rstd, const T* __restrict__ dy, long long lddy, const T* add,
+                                                                long long ldadd, int R, int C, T* dx, long long lddx, int blocks, float* dgamma, float* dbeta,
+                                                                int acc) {
+  if ((int)blockIdx.x < blocks) {
+    ln_bwd_rows<T, L, NV, false>(x, ldx, gamma, mean, rstd, dy, lddy, add, ldadd, R, C, dx, lddx, nullptr, blocks);
+    return;
+  }
+  __shared__ float sg[8][32], sb[8][32];
+  const int c = ((int)blockIdx.x - blocks) * 32 + (threadIdx.x & 31), sl = threadIdx.x >> 5;
+  float g = 0.f, b = 0.f;
+  if (c < C) {
+#pragma unroll 8
+    for (int row = sl; row < R; row += 8) {
+      const float d = TkVec<T>::load(dy + row * lddy + c);
+      g += d * ((TkVec<T>::load(x + row * ldx + c) - mean[row]) * rstd[row]);
+      b += d;
+    }
+  }
+  sg[sl][threadIdx.x & 31] = g; sb[sl][threadIdx.x & 31] = b;
+  __syncthreads();
+  if (sl < 2 && c < C) {
+    float* to = sl ? dbeta : dgamma;
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += sl ? sb[k][threadIdx.x & 31] : sg[k][threadIdx.x & 31];
+    if (to) to[c] = acc ? to[c] + t : t;
+  }
+}
+
 // Rows too long for registers: the block reads its row twice (the second time from L2) and adds into its own partial row in memory; every channel of
 // it belongs to one lane, so no other thread touches it.
 template <typename T, bool WG>
@@ -327,7 +366,7 @@ __global__ void __launch_bounds__(1024) layernorm_wsum_kernel(const float* __res
 // Row form: the smallest group of lanes that holds a row in one vector each (8, 16, 32 or a whole wave up to 512 channels: 64-channel rows on whole
 // waves ran at 0.75 TB/s, seven lanes of eight idle), a wave up to 4 vectors a lane (2048 channels; backward, which keeps more state: 3), then four
 // waves, eight waves (16384 channels), streamed beyond.  Few rows (fewer blocks than CUs at four rows a block) go to four waves each: 128 rows of
-// 2048 fp32, one layer of a latent batch, took 5.0 + 8.6 us with one wave a row, 4.0 + 4.9 with four.
+// 2048 fp32, one layer of a latent batch, took 5.0 us forward with one wave a row, 4.0 with four.
 struct LnForm { int lanes, nv; };
 static LnForm ln_form(int R, int C, bool bwd) {
   const int nv = C / 8;
@@ -350,6 +389,9 @@ static int ln_blocks(int R, int C) {
   const int want = cdiv(R, ln_rows_per_block(f)), most = f.lanes == 512 ? 256 : f.nv == 1 ? 1024 : 512;
   return want < most ? want : most;
 }
+// One launch up to 1024 rows: reading x and dy of 32 columns in 8 slices takes no longer than the row blocks beside it, and a launch less counts (2048 channels bf16,
+// 512 rows 11.6 -> 7.0 us, 1024 rows 16.1 -> 10.4; 2048 rows 18.4 -> 23.4).  The workspace is asked for all the same: what a caller has to hold does not change with this rule.
+static bool ln_few(int R, int C) { return R <= 1024 && ln_form(R, C, true).lanes <= 256; }
 size_t k_layernorm_workspace_bytes(int R, int C) { return R > 0 && C > 0 ? (size_t)ln_blocks(R, C) * 2 * C * sizeof(float) : 0; }
 
 #define LN_FORMS(X, X4, X0)                                                                                       \
@@ -389,6 +431,18 @@ template <typename T, bool WG> static void ln_bwd(const void* x, long long ldx, 
 #undef LN_ARGS
 }
 
+template <typename T> static void ln_bwd_few(const void* x, long long ldx, const float* gamma, const float* mean, const float* rstd, const void* dy, long long lddy,
+                                             const void* add, long long ldadd, int R, int C, void* dx, long long lddx, float* dgamma, float* dbeta, int acc, hipStream_t st) {
+  const LnForm f = ln_form(R, C, true);
+  const int blocks = ln_blocks(R, C);
+#define LN_X(W, V)                                                                                                                                             \
+  if constexpr (W <= 256)                                                                                                                                      \
+    hipLaunchKernelGGL((layernorm_bwd_few_kernel<T, W, V>), dim3(blocks + cdiv(C, 32)), dim3(256), 0, st, (const T*)x, ldx, gamma, mean, rstd, (const T*)dy, lddy, \
+                       (const T*)add, ldadd, R, C, (T*)dx, lddx, blocks, dgamma, dbeta, acc)
+  LN_FORMS(LN_X, break, break)
+#undef LN_X
+}
+
 int k_layernorm_fwd(const void* x, long long ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, long long ldy, float* mean, float* rstd,
                     int dtype, hipStream_t st) {
   PDAE_CHECK_ARG(tk_dtype_ok(dtype), "layernorm: dtype must be 0 (fp32) or 1 (bf16), got %d", dtype);
@@ -416,6 +470,11 @@ int k_layernorm_bwd(const void* x, long long ldx, const float* gamma, const floa
                    "layernorm: tensors must be aligned to their element size");
     PDAE_CHECK_ARG(!wg || (ws && ws_bytes >= k_layernorm_workspace_bytes(R, C)), "layernorm_bwd: weight gradients need %zu bytes of workspace (got %zu)",
                    k_layernorm_workspace_bytes(R, C), ws ? ws_bytes : (size_t)0);
+    if (wg && ln_few(R, C)) {
+      if (dtype == PDAE_DT_F32) ln_bwd_few<float>(x, ldx, gamma, mean, rstd, dy, lddy, add, ldadd, R, C, dx, lddx, dgamma, dbeta, acc_param, st);
+      else ln_bwd_few<tk_bf16>(x, ldx, gamma, mean, rstd, dy, lddy, add, ldadd, R, C, dx, lddx, dgamma, dbeta, acc_param, st);
+      return pdae_launch_status("layernorm_bwd");
+    }
     if (dtype == PDAE_DT_F32) {
       if (wg) ln_bwd<float, true>(x, ldx, gamma, mean, rstd, dy, lddy, add, ldadd, R, C, dx, lddx, (float*)ws, st);
       else ln_bwd<float, false>(x, ldx, gamma, mean, rstd, dy, lddy, add, ldadd, R, C, dx, lddx, (float*)ws, st);

@@ -68,6 +68,13 @@ def test_layernorm(H, rows, C, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,C", [(1024, 130), (1025, 130), (1025, 9), (1030, 520), (1030, 1000), (1026, 1500), (1030, 2043), (1027, 4099), (1025, 8192)])
+def test_layernorm_partial_rows(H, rows, C, dtype):
+    """Around 1024 rows: below, blocks of columns add up the weight gradients in the same launch; above, the row blocks leave partial rows for a second one."""
+    test_layernorm(H, rows, C, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_layernorm_strides_offsets_and_optional_arguments(H, dtype):
     rows, C, ld = 37, 203, 260
     k = H.DTYPES[dtype]

@@ -188,14 +188,21 @@ __device__ __forceinline__ void ln_bwd_rows(const T* __restrict__ x, long long l
       }
     if (has) TkVec<T>::store(orow + te, r * (gt - m1 - xt * m2) + (ar ? TkVec<T>::load(ar + te) : 0.f));
   };
-  // two rows in turn, the next one in flight while this one is worked on (L > 64: all waves of the block walk the same rows)
   const long long row0 = (long long)blockIdx.x * RPB + sub;
-  if (row0 < R) fetch(row0, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
-  for (long long row = row0; row < R; row += 2 * step) {
-    if (row + step < R) fetch(row + step, qx[1], qd[1], tx[1], td[1], mu[1], rs[1]);
-    work(row, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
-    if (row + 2 * step < R) fetch(row + 2 * step, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
-    if (row + step < R) work(row + step, qx[1], qd[1], tx[1], td[1], mu[1], rs[1]);
+  if constexpr (sizeof(T) == 4 && L == 512 && WG) {        // a second row of 16384 fp32 channels finds no registers (2000 rows: 126 us spilled, 96 one by one)
+    for (long long row = row0; row < R; row += step) {
+      fetch(row, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
+      work(row, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
+    }
+  } else {
+    // two rows in turn, the next one in flight while this one is worked on (L > 64: all waves of the block walk the same rows)
+    if (row0 < R) fetch(row0, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
+    for (long long row = row0; row < R; row += 2 * step) {
+      if (row + step < R) fetch(row + step, qx[1], qd[1], tx[1], td[1], mu[1], rs[1]);
+      work(row, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
+      if (row + 2 * step < R) fetch(row + 2 * step, qx[0], qd[0], tx[0], td[0], mu[0], rs[0]);
+      if (row + step < R) work(row + step, qx[1], qd[1], tx[1], td[1], mu[1], rs[1]);
+    }
   }
   if constexpr (WG) {
     float* pg = part + (size_t)blockIdx.x * 2 * C;

@@ -35,12 +35,11 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
 
   // this lane's query columns
   mh_bf16x8 Q[QB][KS][NP];
-  int kmax[QB], qrow[QB];
+  int kmax[QB];
   bool live = false;
 #pragma unroll
   for (int a = 0; a < QB; ++a) {
     const int r = row0 + wv * (32 * QB) + a * 32 + li, tq = r / P.GP, hq = hp * P.GP + r % P.GP;
-    qrow[a] = r;
     const bool ok = r < P.R && tq < lq;
     kmax[a] = ok ? (P.causal ? min(lk, tq + off + 1) : lk) : lk;               // rows that do not exist never force the masked path; they are zeroed at the end
     live = live || ok;
@@ -160,9 +159,10 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
     if (it + 1 < te) step(MhInt<1>(), it + 1);
   }
 
+  const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), he = ln >> 5;      // rows anew: kept from above, they are spilled around the loop (QB = 2)
 #pragma unroll
   for (int a = 0; a < QB; ++a) {
-    const int r = qrow[a];
+    const int r = row0 + wv * (32 * QB) + a * 32 + (ln & 31);
     if (r >= P.R) continue;
     const int tq = r / P.GP, hq = hp * P.GP + r % P.GP;
     const float ls = l[a] + __shfl_xor(l[a], 32);
@@ -171,12 +171,12 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
       float* po = P.part + idx * P.D;
       float* ml = P.part + (long long)P.splits * P.units * P.R * P.D + idx * 2;
       const bool any = tq < lq && ls != 0.f;                                   // (NaN counts: it has to reach the output)
-      if (h == 0) { ml[0] = any ? m[a] : -MH_INF; ml[1] = any ? ls : 0.f; }
+      if (he == 0) { ml[0] = any ? m[a] : -MH_INF; ml[1] = any ? ls : 0.f; }
       if (any) {
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-          for (int g = 0; g < 4; ++g) mh_store4<float, WH>(po, d * 32 + g * 8 + h * 4, P.D, O[a][d][g * 4], O[a][d][g * 4 + 1], O[a][d][g * 4 + 2], O[a][d][g * 4 + 3]);
+          for (int g = 0; g < 4; ++g) mh_store4<float, WH>(po, d * 32 + g * 8 + he * 4, P.D, O[a][d][g * 4], O[a][d][g * 4 + 1], O[a][d][g * 4 + 2], O[a][d][g * 4 + 3]);
       }
       continue;
     }
@@ -189,9 +189,9 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
       for (int g = 0; g < 4; ++g) {
         const float x0 = any ? O[a][d][g * 4] * inv : 0.f, x1 = any ? O[a][d][g * 4 + 1] * inv : 0.f;
         const float x2 = any ? O[a][d][g * 4 + 2] * inv : 0.f, x3 = any ? O[a][d][g * 4 + 3] * inv : 0.f;
-        mh_store4<T, WH>(orow, d * 32 + g * 8 + h * 4, P.D, x0, x1, x2, x3);
+        mh_store4<T, WH>(orow, d * 32 + g * 8 + he * 4, P.D, x0, x1, x2, x3);
       }
-    if (P.lse && h == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = any ? (m[a] + __builtin_amdgcn_logf(ls)) * MH_LN2 : -MH_INF;      // (v_log_f32: log2)
+    if (P.lse && he == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = any ? (m[a] + __builtin_amdgcn_logf(ls)) * MH_LN2 : -MH_INF;      // (v_log_f32: log2)
   }
 }
 

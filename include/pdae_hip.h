@@ -317,7 +317,8 @@ int pdae_attn_bwd(const float* qkv, const float* out, const float* lse, const fl
 #define PDAE_BF16 1
 
 /* y = (x - mu) rstd gamma + beta per row of C channels (biased variance, rstd = 1 / sqrt(var + eps)); next to pdae_mlp_modln_* (which fuses the
- * condition scale and SiLU of MLPSkipNet, fp32 only) this is the bare norm.  ldx / ldy: row strides in elements (>= C).  gamma, beta, mean, rstd may be NULL. */
+ * condition scale and SiLU of MLPSkipNet, fp32 only) this is the bare norm.  ldx / ldy: row strides in elements (>= C);
+ * C <= 2^24.  gamma, beta, mean, rstd may be NULL. */
 int pdae_layernorm_fwd(const void* x, int64_t ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, int64_t ldy, float* mean, float* rstd,
                        int dtype, pdae_stream_t stream);
 /* dx = LayerNorm backward (+ add, the identity path around the norm); dgamma / dbeta (+)= sums over the rows, in a fixed order (acc_param selects "+=";
@@ -341,9 +342,11 @@ int pdae_dropout_bwd(const void* dy, int64_t n, float p, uint64_t seed, uint64_t
  * rows of dk / dv behind k_len are 0.  Keys and queries behind the lengths are never read.  Keys that only `causal` hides are read (with finite values
  * their weight is an exact 0; a non-finite value there may reach rows of the same 128-row tile).
  * Strides in elements; channels are contiguous.  Gradients have their tensor's strides (d_o those of o, dq of q, dk of k, dv of v).
- * Limits: D <= 128, Hq a multiple of Hkv, scale > 0.  Sums, softmax statistics and partial results fp32; bf16 tensors multiply in bf16 (probabilities and
+ * No output may overlap an input or another output.  Limits: D <= 128, Hq a multiple of Hkv, scale > 0, token strides below 2^21 elements, fewer than 2^24
+ * workgroups (tiles of 128 rows times heads and samples).  Sums, softmax statistics and partial results fp32; bf16 tensors multiply in bf16 (probabilities and
  * their gradients rounded to bf16 for the second product), fp32 tensors in three exact bf16 planes x six products.  Results are the same bits every run.
- * lse [B][Hq][Tq] (natural log) may be NULL in the forward; the backward needs it and o.  ws: pdae_mha_workspace_bytes(d, backward). */
+ * lse [B][Hq][Tq] (natural log) may be NULL in the forward; the backward needs it and o.  ws: pdae_mha_workspace_bytes(d, backward),
+ * enough for calls with and without lengths. */
 typedef struct pdae_mha_desc {
   int32_t B, Tq, Tk, Hq, Hkv, D, dtype, causal;
   int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];   /* batch, token, head */

@@ -813,13 +813,17 @@ static int mha_params(const pdae_mha_desc* d, int backward, MhaParams& P) {
   PDAE_CHECK_ARG(d->D >= 1 && d->D <= 128, "mha: head width %d is not supported (1 .. 128)", d->D);
   PDAE_CHECK_ARG(d->scale > 0.f && d->scale < 3.0e38f, "mha: scale must be positive and finite, got %g", (double)d->scale);
   PDAE_CHECK_ARG((long long)d->B * d->Hq < (1ll << 30) && d->Tq < (1 << 30) && d->Tk < (1 << 30), "mha: too many heads or tokens");
-  for (int j = 0; j < 3; ++j)
-    for (const int64_t* st : {d->q_stride, d->k_stride, d->v_stride, d->o_stride})
-      PDAE_CHECK_ARG(st[j] >= 0 && st[j] < (1ll << 40), "mha: stride %lld is out of range", (long long)st[j]);
-  // kernels address inside a tile of at most 256 rows (or one row's heads) with 31 bits from a 64-bit tile address
-  PDAE_CHECK_ARG(256 * (d->q_stride[1] > d->k_stride[1] ? d->q_stride[1] : d->k_stride[1]) < (1 << 29) && 256 * (d->v_stride[1] > d->o_stride[1] ? d->v_stride[1] : d->o_stride[1]) < (1 << 29) &&
-                     (long long)d->Hq * d->q_stride[2] < (d->Hq > 1 && d->Tq * (long long)(d->Hq / d->Hkv) <= 128 ? 1ll << 28 : 1ll << 62),
-                 "mha: a token or head stride is too long for one tile (token strides below 2^21 elements)");
+  const int64_t G = d->Hq / d->Hkv;
+  for (const int64_t* st : {d->q_stride, d->k_stride, d->v_stride, d->o_stride}) {
+    const bool query = st == d->q_stride || st == d->o_stride;
+    for (int j = 0; j < 3; ++j) PDAE_CHECK_ARG(st[j] >= 0 && st[j] < (1ll << 40), "mha: stride %lld is out of range", (long long)st[j]);
+    // the kernels address a tile (at most 256 rows of 4-byte elements) with 31 bits from its 64-bit base; where the heads of a group are rows of one tile, these too
+    PDAE_CHECK_ARG(st[1] < (1 << 21), "mha: a token stride of %lld elements is too long (below 2^21)", (long long)st[1]);
+    PDAE_CHECK_ARG((double)d->B * (double)st[0] + (double)(query ? d->Tq : d->Tk) * (double)st[1] + (double)(query ? d->Hq : d->Hkv) * (double)st[2] < 1e17,
+                   "mha: a tensor of strides (%lld, %lld, %lld) is beyond every address", (long long)st[0], (long long)st[1], (long long)st[2]);
+  }
+  PDAE_CHECK_ARG(G == 1 || d->Tq * G > 128 || G * d->q_stride[2] < (1 << 28), "mha: a head stride of %lld elements is too long for %lld heads in a tile",
+                 (long long)d->q_stride[2], (long long)G);
   PDAE_CHECK_ARG(mha_rows_disjoint(d->o_stride, d->B, d->Tq, d->Hq, d->D), "mha: rows of o overlap (strides %lld, %lld, %lld)", (long long)d->o_stride[0],
                  (long long)d->o_stride[1], (long long)d->o_stride[2]);
   if (backward) {
@@ -864,6 +868,11 @@ extern "C" int pdae_mha_bwd(const pdae_mha_desc* d, const void* q, const void* k
                  "mha_bwd: tensors must be aligned to their element size");
   P.q = q; P.k = k; P.v = v; P.o = o; P.lse = const_cast<float*>(lse); P.d_o = d_o; P.dq = dq; P.dk = dk; P.dv = dv; P.q_len = q_len; P.k_len = k_len;
   return k_mha_bwd(P, d->dtype, ws, ws_bytes, S(stream));
+}
+static bool fits_int(const int64_t* i, int n) {
+  for (int k = 0; k < n; ++k)
+    if (i[k] != (int)i[k]) return false;
+  return true;
 }
 static void mha_desc_from(const pdae_op& o, pdae_mha_desc& d) {
   const int64_t* i = o.i;
@@ -970,8 +979,10 @@ static int run_one(const pdae_op& o, pdae_stream_t st) {
       return PDAE_OK;
     }
     case PDAE_OP_LAYERNORM_FWD:
+      PDAE_CHECK_ARG(fits_int(i, 3), "layernorm: R and C must be below 2^31");
       return pdae_layernorm_fwd(p[0], i[3], F(1), F(2), (int)i[0], (int)i[1], (float)f[0], p[3], i[4], FM(4), FM(5), (int)i[2], st);
     case PDAE_OP_LAYERNORM_BWD:
+      PDAE_CHECK_ARG(fits_int(i, 3), "layernorm: R and C must be below 2^31");
       return pdae_layernorm_bwd(p[0], i[3], F(1), F(2), F(3), p[4], i[4], p[5], i[5], (int)i[0], (int)i[1], p[6], i[6], FM(7), FM(8), (int)i[7], p[9], (size_t)i[8],
                                 (int)i[2], st);
     case PDAE_OP_DROPOUT_FWD:
@@ -979,11 +990,13 @@ static int run_one(const pdae_op& o, pdae_stream_t st) {
     case PDAE_OP_DROPOUT_BWD:
       return pdae_dropout_bwd(p[0], i[0], (float)f[0], (uint64_t)i[2], (uint64_t)(uint32_t)i[3] | (uint64_t)i[4] << 32, p[1], (int)i[5], (int)i[1], st);
     case PDAE_OP_MHA_FWD: {
+      PDAE_CHECK_ARG(fits_int(i, 8), "mha: sizes must be below 2^31");
       pdae_mha_desc md;
       mha_desc_from(o, md);
       return pdae_mha_fwd(&md, p[0], p[1], p[2], (const int32_t*)p[5], (const int32_t*)p[6], p[3], FM(4), p[7], (size_t)i[20], st);
     }
     case PDAE_OP_MHA_BWD: {
+      PDAE_CHECK_ARG(fits_int(i, 8), "mha: sizes must be below 2^31");
       pdae_mha_desc md;
       mha_desc_from(o, md);
       return pdae_mha_bwd(&md, p[0], p[1], p[2], (const int32_t*)p[9], (const int32_t*)p[10], p[3], F(4), p[5], p[6], p[7], p[8], p[11], (size_t)i[20], st);

@@ -420,10 +420,15 @@ size_t k_layernorm_workspace_bytes(int R, int C) { return R > 0 && C > 0 ? (size
 template <typename T> static void ln_fwd(const void* x, long long ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, long long ldy,
                                          float* mean, float* rstd, hipStream_t st) {
   const LnForm f = ln_form(R, C, false);
-  const int grid = cdiv(R, ln_rows_per_block(f));
-#define LN_X(W, V) hipLaunchKernelGGL((layernorm_fwd_kernel<T, W, V>), dim3(grid), dim3(LN_THREADS(W)), 0, st, (const T*)x, ldx, gamma, beta, R, C, eps, (T*)y, ldy, mean, rstd)
-  LN_FORMS(LN_X, LN_X(64, 4), LN_X(512, 0))
+  const int per = ln_rows_per_block(f);
+  for (long long r0 = 0; r0 < R; r0 += (long long)per << 22) {                 // (a launch holds fewer than 2^32 threads)
+    const int n = (int)(R - r0 < (long long)per << 22 ? R - r0 : (long long)per << 22);
+#define LN_X(W, V)                                                                                                                                                  \
+  hipLaunchKernelGGL((layernorm_fwd_kernel<T, W, V>), dim3(cdiv(n, per)), dim3(LN_THREADS(W)), 0, st, (const T*)x + r0 * ldx, ldx, gamma, beta, n, C, eps, (T*)y + r0 * ldy, \
+                     ldy, mean ? mean + r0 : nullptr, rstd ? rstd + r0 : nullptr)
+    LN_FORMS(LN_X, LN_X(64, 4), LN_X(512, 0))
 #undef LN_X
+  }
 }
 template <typename T, bool WG> static void ln_bwd(const void* x, long long ldx, const float* gamma, const float* mean, const float* rstd, const void* dy, long long lddy,
                                                   const void* add, long long ldadd, int R, int C, void* dx, long long lddx, float* ws, hipStream_t st) {
@@ -453,7 +458,7 @@ template <typename T> static void ln_bwd_few(const void* x, long long ldx, const
 int k_layernorm_fwd(const void* x, long long ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, long long ldy, float* mean, float* rstd,
                     int dtype, hipStream_t st) {
   PDAE_CHECK_ARG(tk_dtype_ok(dtype), "layernorm: dtype must be 0 (fp32) or 1 (bf16), got %d", dtype);
-  PDAE_CHECK_ARG(R >= 0 && C > 0, "layernorm: need R >= 0 and C > 0 (got %d, %d)", R, C);
+  PDAE_CHECK_ARG(R >= 0 && C > 0 && C <= 1 << 24, "layernorm: need R >= 0 and C > 0, C at most 2^24 (got %d, %d)", R, C);
   PDAE_CHECK_ARG(eps >= 0.f, "layernorm: eps must not be negative");
   PDAE_CHECK_ARG(ldx >= C && ldy >= C, "layernorm: a row stride is shorter than the row (%lld, %lld < %d)", ldx, ldy, C);
   if (R == 0) return PDAE_OK;
@@ -468,12 +473,12 @@ int k_layernorm_bwd(const void* x, long long ldx, const float* gamma, const floa
                     long long ldadd, int R, int C, void* dx, long long lddx, float* dgamma, float* dbeta, int acc_param, void* ws, size_t ws_bytes, int dtype,
                     hipStream_t st) {
   PDAE_CHECK_ARG(tk_dtype_ok(dtype), "layernorm: dtype must be 0 (fp32) or 1 (bf16), got %d", dtype);
-  PDAE_CHECK_ARG(R >= 0 && C > 0, "layernorm: need R >= 0 and C > 0 (got %d, %d)", R, C);
+  PDAE_CHECK_ARG(R >= 0 && C > 0 && C <= 1 << 24, "layernorm: need R >= 0 and C > 0, C at most 2^24 (got %d, %d)", R, C);
   PDAE_CHECK_ARG(ldx >= C && lddy >= C && lddx >= C && (!add || ldadd >= C), "layernorm: a row stride is shorter than the row");
   const bool wg = dgamma || dbeta;
   if (R > 0) {
     PDAE_CHECK_ARG(x && mean && rstd && dy && dx, "layernorm_bwd: null pointer");
-    PDAE_CHECK_ARG(tk_aligned(x, dtype) && tk_aligned(dy, dtype) && tk_aligned(dx, dtype) && tk_aligned(add, dtype),
+    PDAE_CHECK_ARG(tk_aligned(x, dtype) && tk_aligned(dy, dtype) && tk_aligned(dx, dtype) && tk_aligned(add, dtype) && tk_aligned(ws, PDAE_DT_F32),
                    "layernorm: tensors must be aligned to their element size");
     PDAE_CHECK_ARG(!wg || (ws && ws_bytes >= k_layernorm_workspace_bytes(R, C)), "layernorm_bwd: weight gradients need %zu bytes of workspace (got %zu)",
                    k_layernorm_workspace_bytes(R, C), ws ? ws_bytes : (size_t)0);

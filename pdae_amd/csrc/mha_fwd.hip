@@ -458,7 +458,7 @@ int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   mh_fwd_plan(P, dtype, P.q_len || P.k_len);
   const size_t need = mh_fwd_part_floats(P) * sizeof(float);
   PDAE_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "mha_fwd: needs %zu bytes of workspace (got %zu)", need, ws ? ws_bytes : (size_t)0);
-  PDAE_CHECK_ARG(mh_grid(P) < (1ll << 31) && (long long)P.units * P.R < (1ll << 31), "mha_fwd: too many query rows for one launch");
+  PDAE_CHECK_ARG(mh_grid(P) < (1 << 24) && (long long)P.units * P.R < (1ll << 31), "mha_fwd: too many query rows for one launch");
   P.part = (float*)ws;
   const int qb = mh_qb(dtype, P.R, P.D);
   if (mh_token(P, dtype)) {

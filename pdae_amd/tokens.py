@@ -7,8 +7,10 @@ pdae_layernorm_*, pdae_dropout_*, pdae_mha_*).
 
 Each function allocates its outputs, launches on the current stream of the tensors' device (which need not be the current device) and never
 synchronises.  Activations are fp32 or bf16, parameters and their gradients fp32.  Host code that runs the same shapes every step builds op records
-instead (hip.op_layernorm_fwd, ...) and keeps them in a Plan; that is also the form to capture into a graph."""
+instead (hip.op_layernorm_fwd, ...) and keeps them in a Plan; that is also the form to capture into a graph (a backward through autograd can only be
+captured together with its forward, and while no other graph of the same leaves lives).  Gradients of gradients are refused."""
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import hip as H
 
@@ -56,6 +58,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         xr, weight, mean, rstd = ctx.saved_tensors
         with _on_device("layer_norm", xr, dy):
@@ -87,6 +90,7 @@ class _Dropout(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         p, seed, step, layer = ctx.args
         with _on_device("dropout", dy):
@@ -98,13 +102,25 @@ class _Dropout(torch.autograd.Function):
 
 def dropout(x, p, seed, step=0, layer=0, residual=None):
     """(residual +) x with a fraction p of its elements dropped and the rest scaled by 1 / (1 - p).  The mask is a function of (seed, step, layer, element
-    index): equal arguments give equal masks, and the backward regenerates it."""
+    index): equal arguments give equal masks, and the backward regenerates it.  step and layer: 0 .. 2^32 - 1."""
+    if not (0 <= int(step) < 1 << 32 and 0 <= int(layer) < 1 << 32):
+        raise H.PdaeError(f"dropout: step {step} and layer {layer} must lie in [0, 2^32)")
     return _Dropout.apply(x, residual, float(p), int(seed), int(step), int(layer))
 
 
 def _heads(t):
     """[B, T, H, D] with contiguous channels and non-negative strides, else a copy."""
-    return t if t.stride(3) == 1 and min(t.stride()) >= 0 and all(s < 1 << 20 for s in t.stride()[1:3]) else t.contiguous()
+    return t if t.stride(3) == 1 and all(s < 1 << 20 for s in t.stride()[1:3]) else t.contiguous()
+
+
+def _own_rows(t):
+    """No two rows of D channels of t share memory."""
+    extent = t.shape[3]
+    for s, n in sorted((s, n) for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1):
+        if s < extent:
+            return False
+        extent += s * (n - 1)
+    return True
 
 
 class _Attention(torch.autograd.Function):
@@ -118,9 +134,11 @@ class _Attention(torch.autograd.Function):
             for t in (q_len, k_len):
                 if t is not None and (t.dtype != torch.int32 or t.shape != (q.shape[0],) or not t.is_contiguous()):
                     raise H.PdaeError("attention: lengths must be contiguous int32 [B]")
-            # gradients get their tensor's strides, so in training rows must not share memory (a tensor expanded over batch or heads is copied; autograd
-            # sums its copies' gradients)
-            q, k, v = (t.contiguous() if need and 0 in t.stride() else _heads(t) for t in (q, k, v))
+            # gradients get their tensor's strides, so in training rows must not share memory (a tensor expanded over batch or heads, or of sliding windows, is
+            # copied; autograd sums its copies' gradients)
+            q, k, v = (_heads(t) for t in (q, k, v))
+            if need:
+                q, k, v = (t if _own_rows(t) else t.contiguous() for t in (q, k, v))
             B, Tq, Hq, D = q.shape
             o = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
             a = H.Mha(B, Tq, k.shape[1], Hq, k.shape[2], D, dtype=_dtype(q, "attention"), causal=causal, scale=scale, q_stride=q.stride()[:3], k_stride=k.stride()[:3],
@@ -135,6 +153,7 @@ class _Attention(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_o):
         q, k, v, o, lse, q_len, k_len = ctx.saved_tensors
         a = ctx.a

@@ -84,6 +84,36 @@ def test_attention_refusals(H):
     refuses(H, bwd(H.Mha(**good, q_stride=(0, 16, 8))), "rows of dq")
 
 
+def test_sizes_and_strides_beyond_the_kernels_are_refused(H):
+    good = dict(B=2, Tq=4, Tk=4, Hq=2, Hkv=1, D=8)
+    fwd = lambda a: H.op_mha_fwd(a, P, P, P, P)
+    refuses(H, fwd(H.Mha(**good, v_stride=(1 << 30, 1 << 21, 8))), "token stride")
+    refuses(H, fwd(H.Mha(**good, q_stride=(1 << 39, 16, 1 << 30))), "head stride")                # two heads are rows of one tile
+    refuses(H, fwd(H.Mha(**dict(good, B=1 << 20), k_stride=(1 << 39, 8, 8))), "beyond every address")
+    refuses(H, fwd(H.Mha(**dict(good, B=1 << 25, Hq=1))), "too many query rows")
+    refuses(H, H.op_mha_bwd(H.Mha(**dict(good, B=1 << 25, Hq=1)), P, P, P, P, P, P, P, P, P, ws=P, ws_bytes=1 << 60), "too many")
+    refuses(H, fwd(H.Mha(**dict(good, Tq=(1 << 32) + 4))), r"2\^31")                               # (4 if it were cut to 32 bits)
+    refuses(H, H.op_layernorm_fwd(P, P, P, (1 << 32) + 4, 8, 1e-5, P), r"2\^31")
+    refuses(H, H.op_layernorm_bwd(P, P, P, P, P, 4, (1 << 32) + 8, P), r"2\^31")
+    refuses(H, H.op_layernorm_fwd(P, P, P, 4, (1 << 24) + 1, 1e-5, P), r"2\^24")
+    refuses(H, H.op_layernorm_bwd(P, P, P, P, P, 4, 8, P, P, P, P + 2, ws_bytes=1 << 20), "aligned")
+
+
+def test_token_functions_refuse(H):
+    import torch
+    from pdae_amd import tokens
+    x = torch.zeros(2, 8)
+    for f in (lambda: tokens.layer_norm(x), lambda: tokens.dropout(x, 0.1, 0), lambda: tokens.attention(*(torch.zeros(1, 2, 1, 8),) * 3)):
+        with pytest.raises(H.PdaeError, match="no CPU fallback"):
+            f()
+    for k in (dict(step=1 << 32), dict(step=-1), dict(layer=1 << 32)):
+        with pytest.raises(H.PdaeError, match="must lie in"):
+            tokens.dropout(x, 0.1, 0, **k)
+    row = torch.zeros(1, 9, 2, 8)
+    assert tokens._own_rows(row) and tokens._own_rows(row.transpose(1, 2)) and not tokens._own_rows(row.expand(3, 9, 2, 8))
+    assert not tokens._own_rows(row.as_strided((1, 4, 2, 8), (144, 8, 16, 1)))                     # windows that share tokens
+
+
 def test_refused_op_names_its_place(H):
     ops = H.ops_array([H.op_dropout_fwd(None, None, 0, 0.1, None), H.op_dropout_fwd(P, None, 8, 2.0, P)])
     with pytest.raises(H.PdaeError, match=r"op 1 \(kind %d\)" % H.OP_DROPOUT_FWD):

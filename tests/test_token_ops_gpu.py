@@ -74,6 +74,18 @@ def test_layernorm_partial_rows(H, rows, C, dtype):
     test_layernorm(H, rows, C, dtype)
 
 
+def test_layernorm_more_rows_than_one_launch_holds(H):
+    """2^22 blocks of 32 rows and five more rows; the statistics and rows around the seam and at the end."""
+    rows, C = (32 << 22) + 5, 2
+    x = torch.randn(rows, C, device=DEV, dtype=BF16)
+    y, mean = torch.full_like(x, float("nan")), torch.full((rows,), float("nan"), device=DEV)
+    H.run(H.op_layernorm_fwd(x, None, None, rows, C, 1e-5, y, mean, dtype=H.DT_BF16))
+    for at in (0, rows - 37):
+        ref = R.layer_norm(x[at:at + 37].cpu(), None, None, 1e-5)
+        R.within(y[at:at + 37], ref["y"], "y"); R.within(mean[at:at + 37], ref["mean"], "mean")
+    assert bool(torch.isfinite(mean).all())
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_layernorm_strides_offsets_and_optional_arguments(H, dtype):
     rows, C, ld = 37, 203, 260

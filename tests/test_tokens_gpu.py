@@ -135,6 +135,34 @@ def test_functions_take_views_broadcasts_and_expanded_gradients():
         assert not tokens.attention(qd, kd.expand(3, -1, -1, -1), vd.expand(3, -1, -1, -1)).requires_grad
 
 
+def test_attention_over_sliding_windows_of_one_tensor():
+    """Keys whose rows share memory (overlapping windows): read in place without gradients, copied for them; the gradient sums what the windows share."""
+    from pdae_amd import tokens
+    q, base = rn(1, 3, 6, 2, 16), rn(2, 10, 2, 16)
+    windows = lambda t: t.as_strided((3, 6, 2, 16), (64, 32, 16, 1))                                  # two tokens further each: windows share four of six
+    qd, bd = q.to(DEV).requires_grad_(True), base.to(DEV).requires_grad_(True)
+    o = tokens.attention(qd, windows(bd), windows(bd))
+    with torch.no_grad():
+        assert torch.equal(o, tokens.attention(qd, windows(bd), windows(bd)))
+    o.square().sum().backward()
+    q6, b6 = q.double().requires_grad_(True), base.double().requires_grad_(True)
+    w6 = torch.stack([b6[2 * i:2 * i + 6] for i in range(3)])
+    s = torch.einsum("bihd,bjhd->bhij", q6, w6) / 4.0
+    torch.einsum("bhij,bjhd->bihd", torch.softmax(s, -1), w6).square().sum().backward()
+    assert rel_err(qd.grad, q6.grad) < 1e-5 and rel_err(bd.grad, b6.grad) < 1e-5
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "dropout", "attention"])
+def test_gradients_of_gradients_are_refused(name):
+    """The backward is one kernel that autograd does not see into: a second derivative would silently miss terms."""
+    from pdae_amd import tokens
+    x = rn(3, 1, 5, 2, 16).to(DEV).requires_grad_(True)
+    y = {"layer_norm": lambda: tokens.layer_norm(x), "dropout": lambda: tokens.dropout(x, 0.3, 1), "attention": lambda: tokens.attention(x, x, x)}[name]()
+    g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.square().sum().backward()
+
+
 def test_functions_refuse_what_they_cannot_do():
     from pdae_amd import tokens
     from pdae_amd.hip import PdaeError

@@ -346,6 +346,54 @@ def test_attention_lengths_outside_the_tensor_are_cut(H):
     assert all(torch.equal(x, y) for x, y in zip(*res))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Tq", [1, 150])
+def test_attention_offsets_beyond_32_bits(H, Tq, dtype):
+    """Keys 2^20 elements apart: offsets pass 2^31 elements inside one sample's cache.  The same bits as from a dense copy."""
+    Tk, Hq, Hkv, D, st = 2100, 4, 2, 64, 1 << 20
+    q, g = rn(1, 1, Tq, Hq, D, dtype=dtype).to(DEV), rn(2, 1, Tq, Hq, D, dtype=dtype).to(DEV)
+    kv = rn(3, 2, 1, Tk, Hkv, D, dtype=dtype).to(DEV)
+    wide = lambda: torch.empty(Tk * st, dtype=dtype, device=DEV).as_strided((1, Tk, Hkv, D), (Tk * st, st, D, 1))
+    outs = []
+    for far in (False, True):
+        k, dk = (wide(), wide()) if far else (torch.empty(1, Tk, Hkv, D, dtype=dtype, device=DEV) for _ in range(2))
+        v, dv = (t.as_strided(t.shape, t.stride(), 4096) if far else torch.empty_like(t) for t in (k, dk))     # v lies in the gaps of k
+        k.copy_(kv[0]); v.copy_(kv[1])
+        a = H.Mha(1, Tq, Tk, Hq, Hkv, D, dtype=H.DTYPES[dtype], causal=True, k_stride=k.stride()[:3], v_stride=v.stride()[:3])
+        o, dq, lse, ws = torch.empty_like(q), torch.empty_like(q), torch.empty(1, Hq, Tq, device=DEV), ws_of(a.ws_bytes(True))
+        H.run(H.op_mha_fwd(a, q, k, v, o, lse=lse, ws=ws))
+        H.run(H.op_mha_bwd(a, q, k, v, o, lse, g, dq, dk, dv, ws=ws))
+        outs.append([t.contiguous().clone() for t in (o, lse, dq, dk, dv)])
+        assert torch.equal(k, kv[0]) and torch.equal(v, kv[1])
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Tq", [3, 200])
+def test_attention_keeps_a_bad_row_to_itself_and_shows_a_bad_key(H, Tq, dtype):
+    """NaN in a query makes that row NaN and no other; NaN in a visible key or value reaches every row that sees it."""
+    q, k, v = rn(1, 1, Tq, 2, 64, dtype=dtype), rn(2, 1, 300, 2, 64, dtype=dtype), rn(3, 1, 300, 2, 64, dtype=dtype)
+    ref = R.attention(q, k, v)
+    a = H.Mha(1, Tq, 300, 2, 2, 64, dtype=H.DTYPES[dtype])
+
+    def run(q, k, v):
+        o = torch.empty(q.shape, dtype=dtype, device=DEV)
+        H.run(H.op_mha_fwd(a, q.to(DEV), k.to(DEV), v.to(DEV), o, ws=ws_of(a.ws_bytes())))
+        return o.cpu()
+    bad = q.clone()
+    bad[0, 1, 0, 5] = float("nan")
+    o = run(bad, k, v)
+    assert bool(torch.isnan(o[0, 1, 0]).all())
+    o[0, 1, 0] = ref["o"][0][0, 1, 0].to(dtype)
+    R.within(o, ref["o"], "o")
+    for t in (k, v):
+        bad = t.clone()
+        bad[0, 299, 1] = float("nan")
+        o = run(q, *((bad, v) if t is k else (k, bad)))
+        assert bool(torch.isnan(o[:, :, 1]).all())
+        R.within(o[:, :, :1], tuple(x[:, :, :1] for x in ref["o"]), "o")
+
+
 def test_attention_agrees_with_the_fused_image_attention(H):
     """The same qkv tensor through pdae_attn_fwd / _bwd (64 .. 256 tokens) and through the general kernels by strides, both channel orders."""
     N, T, C, heads = 2, 64, 128, 2

@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
   }
   if (tq >= P.Tq) return;
   if (P.splits > 1) {
-    mh_put<float, DB, WH>(dQ, P.scale, ok, P.part + ((long long)split * P.B * P.Hq * P.Tq + row) * P.D, P.D, h);
+    if (tq < lq) mh_put<float, DB, WH>(dQ, P.scale, ok, P.part + ((long long)split * P.B * P.Hq * P.Tq + row) * P.D, P.D, h);
   } else {
     mh_put<T, DB, WH>(dQ, P.scale, ok, (T*)P.dq + b * P.qb + (long long)tq * P.qt + (long long)hq * P.qh, P.D, h);
   }
@@ -337,24 +337,26 @@ __global__ void __launch_bounds__(256, OCC) mha_dkv_kernel(const MhaParams P) {
     mh_arrive<decltype(sq)::DMA>();
     __syncthreads();
   }
-  if (key >= P.Tk) return;
+  const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), he = ln >> 5, ke = kw + (ln & 31);      // (anew: no register has to hold them in the loop)
+  const bool in = ke < lk;
   if (P.splits > 1) {
+    if (!in) return;                                                           // (the join writes the zeros behind the length)
     const long long n = (long long)P.B * P.Hkv * P.Tk;
-    float* row = P.part + ((long long)split * 2 * n + (long long)unit * P.Tk + key) * P.D;
-    mh_put<float, DB, WH>(dK, P.scale, ok, row, P.D, h);
-    mh_put<float, DB, WH>(dV, 1.f, ok, row + n * P.D, P.D, h);
-  } else {
-    mh_put<T, DB, WH>(dK, P.scale, ok, (T*)P.dk + b * P.kb + (long long)key * P.kt + (long long)hk * P.kh, P.D, h);
-    mh_put<T, DB, WH>(dV, 1.f, ok, (T*)P.dv + b * P.vb + (long long)key * P.vt + (long long)hk * P.vh, P.D, h);
+    float* row = P.part + ((long long)split * 2 * n + (long long)unit * P.Tk + ke) * P.D;
+    mh_put<float, DB, WH>(dK, P.scale, true, row, P.D, he);
+    mh_put<float, DB, WH>(dV, 1.f, true, row + n * P.D, P.D, he);
+  } else if (ke < P.Tk) {
+    mh_put<T, DB, WH>(dK, P.scale, in, (T*)P.dk + b * P.kb + (long long)ke * P.kt + (long long)hk * P.kh, P.D, he);
+    mh_put<T, DB, WH>(dV, 1.f, in, (T*)P.dv + b * P.vb + (long long)ke * P.vt + (long long)hk * P.vh, P.D, he);
   }
 }
 
 // out[b][t][h][d ..] = sum over splits of part[s][(b, h, t)][d ..], in order; `step`: floats between two ranges.  V channels a thread.  blockIdx.y: which
-// of two tensors (their partials lie behind one another).
+// of two tensors (their partials lie behind one another).  Rows behind their length have no partials: zeros.
 struct MhaJoinTo { void* p; long long sb, st, sh; };
 template <typename T, int V>
-__global__ void __launch_bounds__(256) mha_bwd_join_kernel(const float* __restrict__ part, long long step, int splits, MhaJoinTo to0, MhaJoinTo to1, int H, int Tn, int D,
-                                                           long long rows) {
+__global__ void __launch_bounds__(256) mha_bwd_join_kernel(const float* __restrict__ part, long long step, int splits, MhaJoinTo to0, MhaJoinTo to1, const int* len,
+                                                           int H, int Tn, int D, long long rows) {
   const MhaJoinTo to = blockIdx.y ? to1 : to0;
   const int dv = D / V;
   const long long e = (long long)blockIdx.x * 256 + threadIdx.x, row = e / dv;
@@ -364,8 +366,9 @@ __global__ void __launch_bounds__(256) mha_bwd_join_kernel(const float* __restri
   float s[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = 0.f;
+  const int ranges = tok < mh_len(len, b, Tn) ? splits : 0;
 #pragma unroll 8
-  for (int k = 0; k < splits; ++k) {
+  for (int k = 0; k < ranges; ++k) {
     float v[V];
     __builtin_memcpy(v, p + k * step, 4 * V);
 #pragma unroll
@@ -414,14 +417,14 @@ template <typename T, int DP, int QT, int OCC, bool WH = true, bool KL = false> 
   hipFuncSetAttribute(reinterpret_cast<const void*>(&mha_dkv_kernel<T, DP, QT, OCC, WH, KL>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   hipLaunchKernelGGL((mha_dkv_kernel<T, DP, QT, OCC, WH, KL>), dim3((unsigned)mh_grid(P)), dim3(256), lds, st, P);
 }
-static void mh_bwd_join(bool bf, const MhaParams& P, long long step, MhaJoinTo to0, MhaJoinTo to1, int n, int H, int Tn, long long rows, hipStream_t st) {
+static void mh_bwd_join(bool bf, const MhaParams& P, long long step, MhaJoinTo to0, MhaJoinTo to1, int n, const int* len, int H, int Tn, long long rows, hipStream_t st) {
   const dim3 grid((unsigned)((rows * P.D / (P.D % 4 ? 1 : 4) + 255) / 256), n);
   if (P.D % 4 == 0) {
-    if (bf) hipLaunchKernelGGL((mha_bwd_join_kernel<tk_bf16, 4>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, H, Tn, P.D, rows);
-    else hipLaunchKernelGGL((mha_bwd_join_kernel<float, 4>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, H, Tn, P.D, rows);
+    if (bf) hipLaunchKernelGGL((mha_bwd_join_kernel<tk_bf16, 4>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, len, H, Tn, P.D, rows);
+    else hipLaunchKernelGGL((mha_bwd_join_kernel<float, 4>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, len, H, Tn, P.D, rows);
   } else {
-    if (bf) hipLaunchKernelGGL((mha_bwd_join_kernel<tk_bf16, 1>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, H, Tn, P.D, rows);
-    else hipLaunchKernelGGL((mha_bwd_join_kernel<float, 1>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, H, Tn, P.D, rows);
+    if (bf) hipLaunchKernelGGL((mha_bwd_join_kernel<tk_bf16, 1>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, len, H, Tn, P.D, rows);
+    else hipLaunchKernelGGL((mha_bwd_join_kernel<float, 1>), grid, dim3(256), 0, st, P.part, step, P.splits, to0, to1, len, H, Tn, P.D, rows);
   }
 }
 
@@ -455,7 +458,7 @@ int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
     if (int e = pdae_launch_status("mha_dq")) return e;
     if (P.splits > 1) {
       const MhaJoinTo to = {P.dq, P.qb, P.qt, P.qh};
-      mh_bwd_join(bf, P, nq * P.D, to, to, 1, P.Hq, P.Tq, nq, st);
+      mh_bwd_join(bf, P, nq * P.D, to, to, 1, P.q_len, P.Hq, P.Tq, nq, st);
     }
   }
   if (P.Tk > 0) {
@@ -475,7 +478,7 @@ int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
       else mh_dkv_go<float, 128, 32, 1>(P, st);
     }
     if (int e = pdae_launch_status("mha_dkv")) return e;
-    if (P.splits > 1) mh_bwd_join(bf, P, 2 * nk * P.D, MhaJoinTo{P.dk, P.kb, P.kt, P.kh}, MhaJoinTo{P.dv, P.vb, P.vt, P.vh}, 2, P.Hkv, P.Tk, nk, st);
+    if (P.splits > 1) mh_bwd_join(bf, P, 2 * nk * P.D, MhaJoinTo{P.dk, P.kb, P.kt, P.kh}, MhaJoinTo{P.dv, P.vb, P.vt, P.vh}, 2, P.k_len, P.Hkv, P.Tk, nk, st);
   }
   return pdae_launch_status("mha_bwd");
 }

@@ -3,7 +3,8 @@
 //
 // Bound: HBM (forward one read and one write of the tensor, backward two reads and one write).  A row is read ONCE and lives in registers between its
 // reductions: L lanes share it (8 .. 64 of a wave, or a block of 256 / 512), NV vectors of eight elements a lane; only rows beyond 16384 channels are
-// streamed again from L2 (NV = 0).  65536 x 1536 bf16: forward 78 us, backward 135 us (5.2 / 4.5 TB/s; a large copy on this chip moves 5.2).
+// streamed again from L2 (NV = 0).  65536 x 1536 bf16: forward 78 us, backward 134 us + 5 for the partial rows
+// (5.2 / 4.5 TB/s; a large copy on this chip moves 5.2).  128 x 2048 fp32: 3.6 + 3.8 us, two launches.
 // The variance is taken from the deviations (two passes over registers), not from E[x^2] - E[x]^2, which loses what a large mean leaves.
 //
 // Weight gradients: every block walks a fixed set of rows and keeps sum dy xh / sum dy of its lanes' own channels in registers; it leaves ONE partial row per

@@ -1,12 +1,19 @@
-// Attention forward for any number of tokens (mha.h): one pass over the keys with a running maximum and sum per query.
+// Attention forward for any number of tokens (mha.h): one pass over the keys with a running reference and sum per query.
 //
 // Workgroup = 4 waves; wave w owns QB * 32 query rows (its Q fragments stay in registers), the four share key / value tiles of KT tokens in LDS, double
-// buffered: the next tile travels from HBM into registers while this one is multiplied, and is stored to the other buffer behind it: one barrier per tile.
-// Per 32 keys x 32 queries: S^T = K Q^T (DP / 16 MFMAs), t = sc2 s, running maximum m in the log2 domain, p = 2^(t - m), O^T += V^T P (DP / 16 MFMAs).
+// buffered: the next tile is on its way while this one is multiplied (bf16 with D a multiple of 8: straight into LDS, else through registers), one barrier a
+// tile.  Per 32 keys x 32 queries: S^T = K Q^T (DP / 16 MFMAs), p = 2^(sc2 s - reference), O^T += V^T P (DP / 16 MFMAs).
 // Every lane holds 16 of a column's 32 scores: the row maximum is a register tree and one exchange with lane ^ 32, the sum stays per lane until the end.
+// The reference is the maximum when it is set, and only moves when a tile's weights outgrow it by MH_GROW: then the accumulators are scaled, else nothing is.
+//
+// Bound: the matrix cores at the chip's power limit.  4 x 16 heads of 128, 4096 tokens, causal, bf16: 302 us (910 TFLOP/s; the library's 8192^3 product runs at
+// 1320), clock 1.63 GHz of 2.4, matrix pipes busy 54 % of the CUs' time, vector instructions 45 %, LDS 27 %, no bank conflicts.  4 x 8 heads of 64, 4096 tokens: 145 us
+// (950).  QB = 2 (64 rows a wave) halves the LDS reads a product and pays at D <= 64, where registers allow it (run back to back 162 us, with
+// QB = 1 173).
+// fp32, 8 x 4 heads of 64, 1024 tokens: 66 us (six products each: 780 TFLOP/s of bf16 work).
 //
 // Few rows (a token or a few per sample against a long cache): query heads that share a key head are rows of ONE tile (GP = G), and the keys are split into
-// ranges (grid `splits`), each leaving an unnormalised partial (O, m, l); mha_join_kernel adds them in a fixed order.
+// ranges (grid `splits`), each leaving an unnormalised partial (O, m, l); the join kernels add them in a fixed order.
 #include "kernels.h"
 #include "mha.h"
 
@@ -197,7 +204,8 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
 
 // At most 32 rows (a token, or a few, of the heads that share a key head), bf16: every wave works for itself on 32 keys at a time, loaded straight into its own LDS,
 // double buffered, without a barrier; the waves of a block take turns through its key range and are joined in LDS at the end.  In the kernel above the
-// 128-row tile would leave three waves without rows, and the fourth's latency per tile would be the block's.
+// 128-row tile would leave three waves without rows, and the fourth's latency per tile would be the block's (24 samples, 32 heads on 8 of 128, ragged caches of up to
+// 8191, with the join: 112 us there, 89 here).  Bound: HBM; full caches of 8192 keys run at 5.1 .. 5.6 TB/s, 2048 keys of 32 key heads at 5.7 .. 6.0.
 template <int DP, int OCC>
 __global__ void __launch_bounds__(256, OCC) mha_token_kernel(const MhaParams P) {
   constexpr int KS = DP / 16, DB = DP / 32, TE = MhTile<1, 32, DP>::ELEMS, OL = DP + 4;

@@ -9,7 +9,7 @@
 // Bound: the matrix cores at the chip's power limit.  4 x 16 heads of 128, 4096 tokens, causal, bf16: dQ 452 us (910 TFLOP/s), dK / dV 581 us (945), clock 1.63 GHz of
 // 2.4, matrix pipes busy 54 / 57 % of the CUs' time, vector instructions 50 / 35 %, LDS 27 / 43 %, no bank conflicts.  fp32, 8 x 4 heads of 64, 1024 tokens: 88 + 111 us.
 // bf16: dQ is off by 2.4e-3 .. 2.5e-3 of its norm where one rounding of the output costs 1.7e-3: dS is rounded for the second product (1.7e-3) and delta comes from the
-// rounded o (up to 0.9e-3); both add up in squares.
+// rounded o (up to 0.9e-3); both add up in squares.  dS in two planes (a product more): 1.8e-3, but 61 -> 72 us in a training pass of 185 (7 padded samples).
 // Few tiles: the summed axis is split into ranges (grid `splits`), every range leaves an fp32 partial, mha_bwd_join_kernel adds them in order.
 // Row validity is decided where rows are staged: queries that do not exist or (causal) see no key come as zeros with lse = +inf, so P = 0 exactly and
 // non-finite values in them reach nothing.

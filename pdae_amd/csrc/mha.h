@@ -59,9 +59,10 @@ __device__ __forceinline__ bool mh_where(const MhaParams& P, int& unit, int& til
 // Ranges of the summed axis of `tokens`.  256 workgroups give every CU one, and a split costs an fp32 partial written, read and joined, and a prologue: full batches
 // are split only below that, into ~512 (one fp32 sample of 4 heads, 1568 tokens, forward and backward: 167 us at 208 workgroups, 143 at 312, 146 at 468).  With lengths
 // the work per workgroup varies by as much as they do, and the longest decides: ~1024.  A range is at least two tiles; with lengths (they are cut unevenly) and for
-// single tokens (a wave takes 32 keys a step) twice that: one sample, 8 key heads, 8192 keys: 11.3 us with ranges of 256, 16.1 with 128.
+// single tokens (a wave takes 32 keys a step) twice that: one sample, 8 key heads, 8192 keys: 11.3 us with ranges of 256, 16.1 with 128.  Up to five bf16 tiles are
+// not worth a join (training, one sample, 8 heads of 128, 256 tokens: 53 us in ranges, 49 without; 323 tokens the same; 383 tokens, 4 heads of 64: 42 and 44).
 static inline int mh_splits(long long wgs, long long tokens, int dtype, bool lengths, bool token = false) {
-  if (wgs <= 0 || (!lengths && wgs >= 256)) return 1;
+  if (wgs <= 0 || (!lengths && wgs >= 256) || (dtype == PDAE_DT_BF16 && tokens <= 320)) return 1;
   const long long s = (lengths ? 1024 : 512) / wgs, most = tokens / ((dtype == PDAE_DT_BF16 ? 128 : 64) * (lengths || token ? 2 : 1));
   return (int)(s > most ? most < 1 ? 1 : most : s < 1 ? 1 : s);
 }

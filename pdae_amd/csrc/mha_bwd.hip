@@ -91,15 +91,24 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
   sk.init(P.kt, P.D); sv.init(P.vt, P.D);
   // bf16: delta from the ROUNDED o is off by 2^-9 sum |dO||O|, which rows over few keys (large |O|) feel as much as all other roundings together.  Tiles that see
   // at most MH_SHORT keys take it exactly, delta = sum_j p dP, in a sweep of its own over those keys, too.
-  if (NP == 1 && nk > 0 && nk <= MH_SHORT) {
+  const bool sweep = NP == 1 && nk > 0 && nk <= MH_SHORT;
+  // tile `it` of the sweep lies in buffer (ntiles - it) & 1, so the loop's first tile, in flight behind the last one, lies in buffer 0
+  const int t0 = sweep ? 0 : tb;
+  if (sweep || tb < te) {
+    unsigned short* to = mh_sm + (sweep ? ntiles & 1 : 0) * 2 * TE;
+    sk.load(kbase, P.kt, t0 * KT, 0, lk, to); sv.load(vbase, P.vt, t0 * KT, 0, lk, to + TE);
+    sk.store(to); sv.store(to + TE);
+  }
+  mh_loads_done();
+  __syncthreads();
+  if (sweep) {
     float acc = 0.f;
     for (int it = 0; it < ntiles; ++it) {
-      __syncthreads();
-      sk.load(kbase, P.kt, it * KT, 0, lk, mh_sm);
-      sv.load(vbase, P.vt, it * KT, 0, lk, mh_sm + TE);
-      sk.store(mh_sm); sv.store(mh_sm + TE);
-      mh_arrive<decltype(sk)::DMA>();
-      __syncthreads();
+      const unsigned short* cur = mh_sm + ((ntiles - it) & 1) * 2 * TE;
+      unsigned short* nxt = mh_sm + ((ntiles - it - 1) & 1) * 2 * TE;
+      const int tn = it + 1 < ntiles ? it + 1 : tb;
+      const bool more = it + 1 < ntiles || tb < te;
+      if (more) { sk.load(kbase, P.kt, tn * KT, 0, lk, nxt); sv.load(vbase, P.vt, tn * KT, 0, lk, nxt + TE); }
 #pragma unroll 1
       for (int kb = 0; kb < KB; ++kb) {
         mh_f32x16 S, E;
@@ -107,9 +116,9 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           mh_bf16x8 A[NP];
-          mh_frag_rows<NP, KT, DP>(mh_sm, kb * 32, ks, li, h, A);
+          mh_frag_rows<NP, KT, DP>(cur, kb * 32, ks, li, h, A);
           mh_mma<NP>(A, Q[ks], S);
-          mh_frag_rows<NP, KT, DP>(mh_sm + TE, kb * 32, ks, li, h, A);
+          mh_frag_rows<NP, KT, DP>(cur + TE, kb * 32, ks, li, h, A);
           mh_mma<NP>(A, G[ks], E);
         }
 #pragma unroll
@@ -118,19 +127,14 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
           acc += it * KT + kb * 32 + 4 * h + (r & 3) + 8 * (r >> 2) < kmax ? x : 0.f;
         }
       }
+      if (more) { sk.store(nxt); sv.store(nxt + TE); }
+      mh_arrive<decltype(sk)::DMA>();
+      __syncthreads();
     }
     acc += __shfl_xor(acc, 32);
     if (ok) del = acc;
-    __syncthreads();
   }
   if (ok && split == 0 && h == 0) P.delta[row] = del;
-  if (tb < te) {
-    sk.load(kbase, P.kt, tb * KT, 0, lk, mh_sm);
-    sv.load(vbase, P.vt, tb * KT, 0, lk, mh_sm + TE);
-    sk.store(mh_sm); sv.store(mh_sm + TE);
-  }
-  mh_loads_done();
-  __syncthreads();
   for (int it = tb; it < te; ++it) {
     const unsigned short* cur = mh_sm + ((it - tb) & 1) * 2 * TE;
     unsigned short* nxt = mh_sm + (((it - tb) & 1) ^ 1) * 2 * TE;

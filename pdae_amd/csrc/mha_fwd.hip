@@ -423,7 +423,11 @@ template <typename T> static void mh_join(const MhaParams& P, hipStream_t st) {
 
 // ---- host: row packing, key ranges
 static bool mh_token(const MhaParams& P, int dtype) { return dtype == PDAE_DT_BF16 && P.R <= 32 && P.D % 8 == 0; }
-static int mh_qb(int dtype, int R, int D) { return dtype == PDAE_DT_BF16 && R > 128 && D <= 64 && D % 8 == 0 ? 2 : 1; }
+// 64 rows a wave where the chip stays full with half the workgroups (4 heads of 64, 256 tokens: 11.8 us that way, 8.2 with 32 rows; 16 x 8 heads of 40, 1024 x 77 tokens: 15.7
+// and 16.5)
+static int mh_qb(const MhaParams& P, int dtype) {
+  return dtype == PDAE_DT_BF16 && P.R > 128 && P.D <= 64 && P.D % 8 == 0 && (long long)P.units * cdiv(P.R, 256) >= 256 ? 2 : 1;
+}
 // Rows of a tile: with few query tokens the G heads that share a key head become rows of one tile, so its keys are read once for all of them.
 // Then, where the tiles do not fill the chip, the keys are split into ranges.
 static void mh_fwd_plan(MhaParams& P, int dtype, bool lengths) {
@@ -431,7 +435,7 @@ static void mh_fwd_plan(MhaParams& P, int dtype, bool lengths) {
   P.HP = P.Hq / P.GP;
   P.R = P.Tq * P.GP;
   P.units = P.B * P.HP;
-  P.tiles = cdiv(P.R, 128 * mh_qb(dtype, P.R, P.D));
+  P.tiles = cdiv(P.R, 128 * mh_qb(P, dtype));
   P.splits = mh_splits((long long)P.units * P.tiles, P.Tk, dtype, lengths, mh_token(P, dtype));
 }
 template <int DP, int OCC> static void mh_token_go(const MhaParams& P, hipStream_t st) {
@@ -468,7 +472,7 @@ int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   PDAE_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "mha_fwd: needs %zu bytes of workspace (got %zu)", need, ws ? ws_bytes : (size_t)0);
   PDAE_CHECK_ARG(mh_grid(P) < (1 << 24) && (long long)P.units * P.R < (1ll << 31), "mha_fwd: too many query rows for one launch");
   P.part = (float*)ws;
-  const int qb = mh_qb(dtype, P.R, P.D);
+  const int qb = mh_qb(P, dtype);
   if (mh_token(P, dtype)) {
     if (P.D <= 32) mh_token_go<32, 4>(P, st);
     else if (P.D <= 64) mh_token_go<64, 2>(P, st);

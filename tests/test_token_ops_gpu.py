@@ -346,6 +346,16 @@ def test_attention_lengths_outside_the_tensor_are_cut(H):
     assert all(torch.equal(x, y) for x, y in zip(*res))
 
 
+@pytest.mark.parametrize("lengths", [False, True])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", [(128, 150, 140, 2, 2, 64), (64, 257, 100, 4, 2, 32), (43, 300, 70, 3, 1, 40), (256, 129, 65, 1, 1, 8), (64, 130, 700, 4, 4, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_attention_that_fills_the_chip(H, shape, causal, lengths):
+    """Enough workgroups for 64 query rows a wave (bf16, D <= 64, more than 128 rows)."""
+    B, Tq, Tk = shape[:3]
+    ln = dict(q_len=[(37 * b) % (Tq + 1) for b in range(B)], k_len=[(53 * b) % (Tk + 1) for b in range(B)]) if lengths else {}
+    check_mha(H, *shape, BF16, causal=causal, junk=lengths, **ln)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("Tq", [1, 150])
 def test_attention_offsets_beyond_32_bits(H, Tq, dtype):

@@ -51,7 +51,7 @@ class _LayerNorm(torch.autograd.Function):
             xr, R, C, ldx = _rows(x)
             _fp32_vector(weight, C, "layer_norm weight"); _fp32_vector(bias, C, "layer_norm bias")
             y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            mean, rstd = torch.empty(R, device=x.device), torch.empty(R, device=x.device)
+            mean, rstd = (torch.empty(R, dtype=torch.float32, device=x.device) for _ in range(2))
             H.run(H.op_layernorm_fwd(xr, weight, bias, R, C, eps, y, mean, rstd, dtype=_dtype(x, "layer_norm"), ldx=ldx))
         ctx.save_for_backward(xr, weight, mean, rstd)
         ctx.has_bias, ctx.shape, ctx.ldx = bias is not None, x.shape, ldx
@@ -64,8 +64,8 @@ class _LayerNorm(torch.autograd.Function):
         with _on_device("layer_norm", xr, dy):
             dr, R, C, ldd = _rows(dy)
             dx = torch.empty(ctx.shape, dtype=xr.dtype, device=xr.device)
-            dg = torch.empty(C, device=xr.device) if weight is not None and ctx.needs_input_grad[1] else None
-            db = torch.empty(C, device=xr.device) if ctx.has_bias and ctx.needs_input_grad[2] else None
+            dg = torch.empty(C, dtype=torch.float32, device=xr.device) if weight is not None and ctx.needs_input_grad[1] else None
+            db = torch.empty(C, dtype=torch.float32, device=xr.device) if ctx.has_bias and ctx.needs_input_grad[2] else None
             ws = torch.empty(H.layernorm_ws_bytes(R, C), dtype=torch.uint8, device=xr.device) if dg is not None or db is not None else None
             H.run(H.op_layernorm_bwd(xr, weight, mean, rstd, dr, R, C, dx, dg, db, ws, dtype=_dtype(xr, "layer_norm"), ldx=ctx.ldx, lddy=ldd))
         return dx, dg, db, None
@@ -143,7 +143,7 @@ class _Attention(torch.autograd.Function):
             o = torch.empty(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
             a = H.Mha(B, Tq, k.shape[1], Hq, k.shape[2], D, dtype=_dtype(q, "attention"), causal=causal, scale=scale, q_stride=q.stride()[:3], k_stride=k.stride()[:3],
                       v_stride=v.stride()[:3], o_stride=o.stride()[:3])
-            lse = torch.empty(B, Hq, Tq, device=q.device) if need else None
+            lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=q.device) if need else None
             n = a.ws_bytes(False)
             ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
             H.run(H.op_mha_fwd(a, q, k, v, o, lse=lse, q_len=q_len, k_len=k_len, ws=ws))

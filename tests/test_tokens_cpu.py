@@ -1,0 +1,57 @@
+"""CPU: what the tensor functions of pdae_amd/tokens.py hand to the kernels -- buffers, their types and how long they live, and which layouts are copied.  Nothing is
+launched: the op records are caught where they would run."""
+import contextlib
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def caught(monkeypatch):
+    """Lets the functions run on CPU tensors: [(op constructor, args, kwargs)] of every record built, `ran` called in place of the launch."""
+    from pdae_amd import tokens
+
+    class Caught(list):
+        def ran(self, op):
+            pass
+    calls = Caught()
+    monkeypatch.setattr(tokens, "_on_device", lambda name, first, *others: contextlib.nullcontext())
+
+    class Hip:
+        def __getattr__(self, name):
+            f = getattr(tokens_hip, name)
+            if not name.startswith("op_"):
+                return f
+
+            def build(*a, **k):
+                calls.append((name, a, k))
+                return f(*a, **k)
+            return build
+
+        def run(self, op, stream=None):
+            calls.ran(op)
+    tokens_hip = tokens.H
+    monkeypatch.setattr(tokens, "H", Hip())
+    return calls
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float16, torch.float64])
+def test_statistics_and_parameter_gradients_are_fp32_under_any_default_type(caught, default):
+    """The kernels write fp32 statistics and parameter gradients: a buffer of torch's default type would be written past its end (bf16) or read as garbage."""
+    from pdae_amd import tokens
+    x = torch.zeros(3, 8, dtype=torch.bfloat16, requires_grad=True)
+    w, b = (torch.ones(8, dtype=torch.float32, requires_grad=True) for _ in range(2))
+    q = torch.zeros(1, 4, 2, 8, dtype=torch.bfloat16, requires_grad=True)
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        y = tokens.layer_norm(x, w, b)
+        y.backward(torch.zeros_like(y))
+        o = tokens.attention(q, q, q)
+        o.backward(torch.zeros_like(o))
+    finally:
+        torch.set_default_dtype(before)
+    args = {n: (a, k) for n, a, k in caught}
+    fp32 = list(args["op_layernorm_fwd"][0][7:9]) + list(args["op_layernorm_bwd"][0][8:10]) + [args["op_mha_fwd"][1]["lse"]]
+    assert len(fp32) == 5 and all(t.dtype == torch.float32 for t in fp32)
+    assert y.dtype == o.dtype == torch.bfloat16 and w.grad.dtype == torch.float32

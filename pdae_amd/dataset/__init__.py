@@ -34,7 +34,7 @@ class SYNTHETIC:
         return self.length
 
     def batch(self, batch_size, device, generator=None):
-        x = torch.rand(batch_size, self.channel, self.size, self.size, device=device, generator=generator) * 2 - 1
+        x = torch.rand(batch_size, self.channel, self.size, self.size, dtype=torch.float32, device=device, generator=generator) * 2 - 1
         gts = ((x + 1) * 127.5).clamp(0, 255).to(torch.uint8).permute(0, 2, 3, 1)
         return {"idx": torch.arange(batch_size), "x_0": x, "gts": gts}
 
@@ -193,7 +193,7 @@ class DeviceImagePipeline:
         batch_size = int(ids.numel())
         Hs, Ws, C = self.images.shape
         S = self.size
-        x0 = torch.empty(batch_size, C, S, S, device=self.device) if out is None else out[:batch_size]
+        x0 = torch.empty(batch_size, C, S, S, dtype=torch.float32, device=self.device) if out is None else out[:batch_size]
         gts = torch.empty(batch_size, S, S, C, dtype=torch.uint8, device=self.device)
         cur = torch.cuda.current_stream(self.device)
         cur.wait_event(slot["ready"])                              # the H2D copy of this slot ran on the side stream

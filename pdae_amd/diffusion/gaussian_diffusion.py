@@ -133,7 +133,7 @@ class GaussianDiffusion:
     def noise_p_sample(self, x_t, t, predicted_noise, learned_range=None, gradient=None, noise=None):   # :112-126 (+ :268-269 with `gradient`)
         """x_{t-1} ~ p(. | x_t): mean from the predicted noise (shifted by shift_coef[t] * gradient when given), fixed-small or learned
         variance, no noise where t == 0.  One kernel; `noise` may be injected."""
-        noise = torch.randn(x_t.shape, device=x_t.device) if noise is None else noise
+        noise = torch.randn(x_t.shape, dtype=torch.float32, device=x_t.device) if noise is None else noise
         cx, ce, cs, lv0 = self._rows(t, "noise_posterior_mean_x_t_coef", "noise_posterior_mean_noise_coef", "shift_coef",
                                      "posterior_log_variance_clipped")
         coef = torch.stack([cx, ce, cs, (t != 0).to(torch.float32), lv0, self._log_betas.gather(0, t)], 1)
@@ -286,7 +286,7 @@ class GaussianDiffusion:
         of the steps (:415).  `z_T` may be injected (already clamped or not)."""
         cfg = self.latent_diffusion_config
         if z_T is None:
-            z_T = torch.randn((x_T.shape[0], latent_denoise_fn.input_channel), device=self.device)
+            z_T = torch.randn((x_T.shape[0], latent_denoise_fn.input_channel), dtype=torch.float32, device=self.device)
         z = self._ddim(latent_ddim_style, cfg["_ac_host"]).latent_ddim_sample_loop(latent_denoise_fn, z_T.clamp(-1.0, 1.0))
         return self.representation_learning_ddim_sample(decoder_ddim_style, None, decoder, None, x_T, self.denormalize(z, latents_mean, latents_std),
                                                         stop_percent=0.3)

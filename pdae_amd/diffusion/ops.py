@@ -24,8 +24,8 @@ class _Loss(torch.autograd.Function):
         eps, noise = _c(eps), _c(noise)
         g = _c(g) if g is not None else None
         N = eps.shape[0]
-        loss = torch.empty(1, device=eps.device)
-        ws = torch.empty(2048, device=eps.device)
+        loss = torch.empty(1, dtype=torch.float32, device=eps.device)
+        ws = torch.empty(2048, dtype=torch.float32, device=eps.device)
         deps = torch.empty_like(eps) if ctx.needs_input_grad[0] else None
         dg = torch.empty_like(g) if (g is not None and ctx.needs_input_grad[1]) else None
         H.run(H.op_loss(noise, eps, g, t, tc, tw, N, eps.numel() // N, loss, ws, deps=deps, dg=dg, l1=int(l1)))

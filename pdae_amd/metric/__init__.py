@@ -32,9 +32,9 @@ def ssim_mse(img1, img2, denormalize=False, want_ssim=True, want_mse=True):
     img1, img2 = img1.float(), img2.float()
     N, C, Hh, W = img1.shape
     L = H.lib()
-    ws = torch.empty(max(L.pdae_ssim_mse_workspace_bytes(N, C, Hh, W) // 4, 1), device=img1.device)
-    s = torch.empty(N, device=img1.device) if want_ssim else None
-    m = torch.empty(N, device=img1.device) if want_mse else None
+    ws = torch.empty(max(L.pdae_ssim_mse_workspace_bytes(N, C, Hh, W) // 4, 1), dtype=torch.float32, device=img1.device)
+    s = torch.empty(N, dtype=torch.float32, device=img1.device) if want_ssim else None
+    m = torch.empty(N, dtype=torch.float32, device=img1.device) if want_mse else None
     mul, add = (0.5, 0.5) if denormalize else (1.0, 0.0)
     sa, sb = (ctypes.c_int64 * 4)(*img1.stride()), (ctypes.c_int64 * 4)(*img2.stride())
     rc = L.pdae_ssim_mse(img1.data_ptr(), sa, img2.data_ptr(), sb, N, C, Hh, W, mul, add, _WINDOW, s.data_ptr() if want_ssim else None,

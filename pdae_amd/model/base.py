@@ -60,7 +60,7 @@ class PlannedNet(FlatModule):
 
     def _dummy_leaf(self):
         if self._dummy is None:
-            object.__setattr__(self, "_dummy", torch.zeros(1, device=self.device, requires_grad=True))
+            object.__setattr__(self, "_dummy", torch.zeros(1, dtype=torch.float32, device=self.device, requires_grad=True))
         return self._dummy
 
     def _wants_grad(self):

@@ -76,7 +76,7 @@ class MLPSkipNet(PlannedNet):
         for i in range(n - 1):
             for nm in ("linear", "linear_emb"):
                 w = self.P[f"layers.{i}.{nm}.weight"]
-                w.copy_(torch.randn(w.shape, device=w.device) * (2.0 / w.shape[1]) ** 0.5)
+                w.copy_(torch.randn(w.shape, dtype=torch.float32, device=w.device) * (2.0 / w.shape[1]) ** 0.5)
 
     # ------------------------------------------------------------------ graph
     def _emit_forward(self, B, x, t, dropout=0.0):

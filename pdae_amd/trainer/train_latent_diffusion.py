@@ -59,7 +59,7 @@ class LatentDiffusionTrainer(_LoopMixin):
         elif not self.allow_random_init:
             raise FileNotFoundError(f"inferred latents {lat!r} not found (pass --allow_random_init to train on N(0,1) stand-in statistics)")
         else:
-            self.latents_mean, self.latents_std = torch.zeros(d, device=self.device), torch.ones(d, device=self.device)
+            self.latents_mean, self.latents_std = torch.zeros(d, dtype=torch.float32, device=self.device), torch.ones(d, dtype=torch.float32, device=self.device)
         oc = c["optimizer_config"]
         name = oc.get("name", "Adam")
         if name not in ("Adam", "AdamW"):

@@ -45,7 +45,7 @@ class _LoopMixin:
     def _run(self, one_step, samples_per_step):
         rc = self.config["runner_config"]
         display = int(rc["display_steps"])
-        acc, acc_n = torch.zeros(1, device=self.device), 0
+        acc, acc_n = torch.zeros(1, dtype=torch.float32, device=self.device), 0
         t_top = time.time()
         n_it = int(rc.get("num_iterations", 1))
         while self.max_steps is None or self.step < self.max_steps:

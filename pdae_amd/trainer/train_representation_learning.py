@@ -104,7 +104,7 @@ class RepresentationLearningTrainer:
     def train(self):
         rc = self.config["runner_config"]
         display, n_it = int(rc["display_steps"]), int(rc["num_iterations"])
-        acc, acc_n = torch.zeros(1, device=self.device), 0
+        acc, acc_n = torch.zeros(1, dtype=torch.float32, device=self.device), 0
         t_top = time.time()
         gen = torch.Generator(device=self.device)
         gen.manual_seed(int(time.time()) + self.global_rank)

@@ -55,3 +55,23 @@ def test_statistics_and_parameter_gradients_are_fp32_under_any_default_type(caug
     fp32 = list(args["op_layernorm_fwd"][0][7:9]) + list(args["op_layernorm_bwd"][0][8:10]) + [args["op_mha_fwd"][1]["lse"]]
     assert len(fp32) == 5 and all(t.dtype == torch.float32 for t in fp32)
     assert y.dtype == o.dtype == torch.bfloat16 and w.grad.dtype == torch.float32
+
+
+def test_no_buffer_of_the_package_takes_torchs_default_type():
+    """Every kernel argument has a fixed element type: a factory call that names none follows torch.set_default_dtype, and the kernel writes past the buffer."""
+    import ast
+    import os
+    import pdae_amd
+    root, bad = os.path.dirname(pdae_amd.__file__), []
+    for folder, _, files in os.walk(root):
+        for f in files:
+            if not f.endswith(".py"):
+                continue
+            path = os.path.join(folder, f)
+            with open(path) as fh:
+                tree = ast.parse(fh.read())
+            for n in ast.walk(tree):
+                if isinstance(n, ast.Call) and isinstance(n.func, ast.Attribute) and isinstance(n.func.value, ast.Name) and n.func.value.id == "torch" and \
+                        n.func.attr in ("empty", "zeros", "ones", "full", "rand", "randn", "empty_strided") and "dtype" not in [k.arg for k in n.keywords]:
+                    bad.append(f"{os.path.relpath(path, root)}:{n.lineno}")
+    assert not bad, bad

@@ -84,9 +84,9 @@ class _Dropout(torch.autograd.Function):
             xc = x.contiguous()
             if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
                 raise H.PdaeError("dropout: the residual must have x's shape and type")
+            rc = None if residual is None else residual.contiguous()           # (a name of its own: the record holds its address only)
             y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            H.run(H.op_dropout_fwd(xc, None if residual is None else residual.contiguous(), x.numel(), p, y, seed=seed, offset=step, layer=layer,
-                                   dtype=_dtype(x, "dropout")))
+            H.run(H.op_dropout_fwd(xc, rc, x.numel(), p, y, seed=seed, offset=step, layer=layer, dtype=_dtype(x, "dropout")))
         return y
 
     @staticmethod

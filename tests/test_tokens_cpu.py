@@ -75,3 +75,20 @@ def test_no_buffer_of_the_package_takes_torchs_default_type():
                         n.func.attr in ("empty", "zeros", "ones", "full", "rand", "randn", "empty_strided") and "dtype" not in [k.arg for k in n.keywords]:
                     bad.append(f"{os.path.relpath(path, root)}:{n.lineno}")
     assert not bad, bad
+
+
+def test_contiguous_copies_live_until_the_launch(caught):
+    """A record holds addresses: a copy that is dropped before the record runs may be handed to another thread of the same stream, which then writes into it."""
+    import weakref
+
+    from pdae_amd import tokens
+    base = torch.randn(8, 6)
+    refs = []
+
+    def ran(op):
+        while caught:                                     # (the fixture's own hold on the arguments ends here)
+            refs.extend(weakref.ref(t) for t in caught.pop()[1] if isinstance(t, torch.Tensor))
+        assert refs and all(r() is not None for r in refs)
+    caught.ran = ran
+    tokens.dropout(base.t(), 0.1, 1, residual=(base * 2).t())
+    assert len(refs) == 3

@@ -814,28 +814,35 @@ static int mha_params(const pdae_mha_desc* d, int backward, MhaParams& P) {
   PDAE_CHECK_ARG(d->scale > 0.f && d->scale < 3.0e38f, "mha: scale must be positive and finite, got %g", (double)d->scale);
   PDAE_CHECK_ARG((long long)d->B * d->Hq < (1ll << 30) && d->Tq < (1 << 30) && d->Tk < (1 << 30), "mha: too many heads or tokens");
   const int64_t G = d->Hq / d->Hkv;
-  for (const int64_t* st : {d->q_stride, d->k_stride, d->v_stride, d->o_stride}) {
-    const bool query = st == d->q_stride || st == d->o_stride;
-    for (int j = 0; j < 3; ++j) PDAE_CHECK_ARG(st[j] >= 0 && st[j] < (1ll << 40), "mha: stride %lld is out of range", (long long)st[j]);
+  // strides by tensor (q, k, v, o); that of an axis with at most one element counts as 0: no address uses it, and such a tensor may carry any
+  int64_t st[4][3];
+  const int64_t* given[4] = {d->q_stride, d->k_stride, d->v_stride, d->o_stride};
+  for (int t = 0; t < 4; ++t) {
+    const bool query = t == 0 || t == 3;
+    const int n[3] = {d->B, query ? d->Tq : d->Tk, query ? d->Hq : d->Hkv};
+    for (int j = 0; j < 3; ++j) {
+      st[t][j] = n[j] > 1 ? given[t][j] : 0;
+      PDAE_CHECK_ARG(st[t][j] >= 0 && st[t][j] < (1ll << 40), "mha: stride %lld is out of range", (long long)st[t][j]);
+    }
     // the kernels address a tile (at most 256 rows of 4-byte elements) with 31 bits from its 64-bit base; where the heads of a group are rows of one tile, these too
-    PDAE_CHECK_ARG(st[1] < (1 << 21), "mha: a token stride of %lld elements is too long (below 2^21)", (long long)st[1]);
-    PDAE_CHECK_ARG((double)d->B * (double)st[0] + (double)(query ? d->Tq : d->Tk) * (double)st[1] + (double)(query ? d->Hq : d->Hkv) * (double)st[2] < 1e17,
-                   "mha: a tensor of strides (%lld, %lld, %lld) is beyond every address", (long long)st[0], (long long)st[1], (long long)st[2]);
+    PDAE_CHECK_ARG(st[t][1] < (1 << 21), "mha: a token stride of %lld elements is too long (below 2^21)", (long long)st[t][1]);
+    PDAE_CHECK_ARG((double)n[0] * (double)st[t][0] + (double)n[1] * (double)st[t][1] + (double)n[2] * (double)st[t][2] < 1e17,
+                   "mha: a tensor of strides (%lld, %lld, %lld) is beyond every address", (long long)st[t][0], (long long)st[t][1], (long long)st[t][2]);
   }
-  PDAE_CHECK_ARG(G == 1 || d->Tq * G > 128 || G * d->q_stride[2] < (1 << 28), "mha: a head stride of %lld elements is too long for %lld heads in a tile",
-                 (long long)d->q_stride[2], (long long)G);
-  PDAE_CHECK_ARG(mha_rows_disjoint(d->o_stride, d->B, d->Tq, d->Hq, d->D), "mha: rows of o overlap (strides %lld, %lld, %lld)", (long long)d->o_stride[0],
-                 (long long)d->o_stride[1], (long long)d->o_stride[2]);
+  PDAE_CHECK_ARG(G == 1 || d->Tq * G > 128 || G * st[0][2] < (1 << 28), "mha: a head stride of %lld elements is too long for %lld heads in a tile",
+                 (long long)st[0][2], (long long)G);
+  PDAE_CHECK_ARG(mha_rows_disjoint(st[3], d->B, d->Tq, d->Hq, d->D), "mha: rows of o overlap (strides %lld, %lld, %lld)", (long long)st[3][0], (long long)st[3][1],
+                 (long long)st[3][2]);
   if (backward) {
-    PDAE_CHECK_ARG(mha_rows_disjoint(d->q_stride, d->B, d->Tq, d->Hq, d->D), "mha: rows of dq (the strides of q) overlap");
-    PDAE_CHECK_ARG(mha_rows_disjoint(d->k_stride, d->B, d->Tk, d->Hkv, d->D), "mha: rows of dk (the strides of k) overlap");
-    PDAE_CHECK_ARG(mha_rows_disjoint(d->v_stride, d->B, d->Tk, d->Hkv, d->D), "mha: rows of dv (the strides of v) overlap");
+    PDAE_CHECK_ARG(mha_rows_disjoint(st[0], d->B, d->Tq, d->Hq, d->D), "mha: rows of dq (the strides of q) overlap");
+    PDAE_CHECK_ARG(mha_rows_disjoint(st[1], d->B, d->Tk, d->Hkv, d->D), "mha: rows of dk (the strides of k) overlap");
+    PDAE_CHECK_ARG(mha_rows_disjoint(st[2], d->B, d->Tk, d->Hkv, d->D), "mha: rows of dv (the strides of v) overlap");
   }
   memset(&P, 0, sizeof(P));
   P.B = d->B; P.Tq = d->Tq; P.Tk = d->Tk; P.Hq = d->Hq; P.Hkv = d->Hkv; P.G = d->Hq / d->Hkv; P.D = d->D; P.causal = d->causal != 0;
   P.scale = d->scale; P.sc2 = d->scale * MH_LOG2E;
-  P.qb = d->q_stride[0]; P.qt = d->q_stride[1]; P.qh = d->q_stride[2]; P.kb = d->k_stride[0]; P.kt = d->k_stride[1]; P.kh = d->k_stride[2];
-  P.vb = d->v_stride[0]; P.vt = d->v_stride[1]; P.vh = d->v_stride[2]; P.ob = d->o_stride[0]; P.ot = d->o_stride[1]; P.oh = d->o_stride[2];
+  P.qb = st[0][0]; P.qt = st[0][1]; P.qh = st[0][2]; P.kb = st[1][0]; P.kt = st[1][1]; P.kh = st[1][2];
+  P.vb = st[2][0]; P.vt = st[2][1]; P.vh = st[2][2]; P.ob = st[3][0]; P.ot = st[3][1]; P.oh = st[3][2];
   return PDAE_OK;
 }
 extern "C" size_t pdae_mha_workspace_bytes(const pdae_mha_desc* d, int backward) {

@@ -1,0 +1,37 @@
+"""CPU: what the C entries of the token operators refuse, and what they must not refuse."""
+import pytest
+
+
+@pytest.fixture(scope="module")
+def H():
+    from pdae_amd.build import build_library
+    build_library(verbose=False)
+    from pdae_amd import hip
+    return hip
+
+
+def refuses(H, op, match):
+    with pytest.raises(H.PdaeError, match=match):
+        H.run(op, stream=0)
+
+
+P = 4096        # stands for a device pointer: every call here ends before a launch
+
+
+def test_strides_of_one_element_axes_are_not_looked_at(H):
+    """A tensor with one sample, token or head may carry any stride there (time-major queries of one token, a slice of a cache): the address never uses it."""
+    far = 1 << 45
+    one = H.Mha(1, 1, 1, 1, 1, 128, **{k + "_stride": (far, far, far) for k in "qkvo"})
+    refuses(H, H.op_mha_fwd(one, None, P, P, P), "null")
+    refuses(H, H.op_mha_bwd(one, P, P, P, P, P, P, None, P, P, ws=P, ws_bytes=1 << 40), "null")
+    # one token of 512 samples, samples inside the token: contiguous, with a token stride of 512 x 32 x 128
+    t = H.Mha(512, 1, 64, 32, 32, 128, dtype=H.DT_BF16, q_stride=(4096, 1 << 21, 128))
+    refuses(H, H.op_mha_fwd(t, None, P, P, P), "null")
+    # a shared key head with one query head has no packed rows
+    g = H.Mha(2, 4, 4, 1, 1, 8, q_stride=(64, 16, 1 << 30))
+    refuses(H, H.op_mha_fwd(g, None, P, P, P), "null")
+    # where the axis is longer the limits stand
+    for k, s in (("q", (4096, 1 << 21, 128)), ("k", (4096, 1 << 21, 128))):
+        refuses(H, H.op_mha_fwd(H.Mha(1, 2, 2, 2, 2, 8, **{k + "_stride": s}), P, P, P, P), "token stride")
+    refuses(H, H.op_mha_fwd(H.Mha(2, 1, 1, 1, 1, 8, v_stride=(far, 1, 1)), P, P, P, P), "out of range")
+    refuses(H, H.op_mha_fwd(H.Mha(1, 1, 4, 2, 1, 8, q_stride=(1, 1, 1 << 27)), P, P, P, P), "head stride")

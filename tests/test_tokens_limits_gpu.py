@@ -39,3 +39,24 @@ def test_results_do_not_depend_on_the_default_type(default):
         torch.set_default_dtype(before)
     for a, c in zip(want, got):
         assert a.dtype == c.dtype and torch.equal(a, c)
+
+
+def test_single_token_queries_with_the_samples_inside_the_token():
+    """[1, B, H, D] seen as [B, 1, H, D]: dense, with a token stride that no address uses."""
+    from pdae_amd import tokens
+    base = rn(1, 1, 512, 32, 128, dtype=BF16)
+    k, v = rn(2, 512, 3, 8, 128, dtype=BF16), rn(3, 512, 3, 8, 128, dtype=BF16)
+    q = base.to(DEV).transpose(0, 1)
+    assert q.stride(1) == 1 << 21 and q.is_contiguous()
+    kd, vd = k.to(DEV), v.to(DEV)
+    plain = torch.empty(512, 1, 32, 128, dtype=BF16, device=DEV).copy_(q)
+    assert plain.stride(1) == 4096
+    got = tokens.attention(q, kd, vd)
+    assert torch.equal(got, tokens.attention(plain, kd, vd))
+    some = slice(200, 203)
+    R.within(got[some], R.attention(base[0, some, None], k[some], v[some])["o"], "o")
+    leaves = [t.clone().requires_grad_(True) for t in (q, kd, vd)]
+    tokens.attention(*leaves).backward(torch.ones_like(got))
+    want = [t.clone().requires_grad_(True) for t in (plain, kd, vd)]
+    tokens.attention(*want).backward(torch.ones_like(got))
+    assert all(torch.equal(a.grad, b.grad) for a, b in zip(leaves, want))

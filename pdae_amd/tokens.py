@@ -108,9 +108,13 @@ def dropout(x, p, seed, step=0, layer=0, residual=None):
     return _Dropout.apply(x, residual, float(p), int(seed), int(step), int(layer))
 
 
-def _heads(t):
-    """[B, T, H, D] with contiguous channels and non-negative strides, else a copy."""
-    return t if t.stride(3) == 1 and all(s < 1 << 20 for s in t.stride()[1:3]) else t.contiguous()
+def _heads(t, group=1):
+    """t ([B, T, H, D]) if the kernels take its strides, else a contiguous copy.  The limits are those of pdae_mha_desc: contiguous channels, token strides
+    below 2^21 elements, and for queries whose `group` heads share a key head as rows of one tile (at most 128 of them) 2^28 over the group."""
+    T, H = t.shape[1:3]
+    if t.stride(3) != 1 or (T > 1 and t.stride(1) >= 1 << 21) or (group > 1 and H > 1 and T * group <= 128 and group * t.stride(2) >= 1 << 28):
+        return t.contiguous()
+    return t
 
 
 def _own_rows(t):
@@ -136,7 +140,7 @@ class _Attention(torch.autograd.Function):
                     raise H.PdaeError("attention: lengths must be contiguous int32 [B]")
             # gradients get their tensor's strides, so in training rows must not share memory (a tensor expanded over batch or heads, or of sliding windows, is
             # copied; autograd sums its copies' gradients)
-            q, k, v = (_heads(t) for t in (q, k, v))
+            q, k, v = _heads(q, q.shape[2] // max(k.shape[2], 1)), _heads(k), _heads(v)
             if need:
                 q, k, v = (t if _own_rows(t) else t.contiguous() for t in (q, k, v))
             B, Tq, Hq, D = q.shape

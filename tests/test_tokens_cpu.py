@@ -92,3 +92,22 @@ def test_contiguous_copies_live_until_the_launch(caught):
     caught.ran = ran
     tokens.dropout(base.t(), 0.1, 1, residual=(base * 2).t())
     assert len(refs) == 3
+
+
+def test_layouts_the_kernels_take_are_not_copied():
+    """A head-major cache has head strides of tokens x channels: only token strides (and packed query heads) are limited in the kernels."""
+    from pdae_amd import tokens
+    meta = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device="meta")
+    cache = meta(2, 8, 8192, 128).transpose(1, 2)
+    assert cache.stride() == (8 << 20, 128, 1 << 20, 1) and tokens._heads(cache) is cache
+    q = meta(2, 32, 1, 128).transpose(1, 2)
+    assert tokens._heads(q, group=4) is q
+    one = meta(1, 512, 32, 128).transpose(0, 1)                                        # the stride of a lone token is no limit
+    assert tokens._heads(one, group=4) is one
+    wide = meta(2, 4, 1 << 21)[:, :, :16].unflatten(2, (2, 8))                         # token stride 2^21: beyond the kernels' tile
+    assert tokens._heads(wide).is_contiguous()
+    apart = torch.empty_strided((1, 4, 2, 8), (0, 8, 1 << 27, 1), device="meta")       # two packed query heads 2^27 apart
+    assert tokens._heads(apart) is apart and tokens._heads(apart, group=2).is_contiguous()
+    many = torch.empty_strided((1, 65, 2, 8), (0, 8, 1 << 27, 1), device="meta")       # 65 x 2 rows: heads are not packed
+    assert tokens._heads(many, group=2) is many
+    assert tokens._heads(meta(2, 4, 8, 2).transpose(2, 3)).is_contiguous()             # channels apart

@@ -60,3 +60,26 @@ def test_single_token_queries_with_the_samples_inside_the_token():
     want = [t.clone().requires_grad_(True) for t in (plain, kd, vd)]
     tokens.attention(*want).backward(torch.ones_like(got))
     assert all(torch.equal(a.grad, b.grad) for a, b in zip(leaves, want))
+
+
+def test_head_major_caches_are_read_in_place():
+    """[B, H, T, D] caches with T D = 2^20 (head strides far beyond the token limit): the bits of the token-major copy, and no copy of the cache."""
+    from pdae_amd import tokens
+    B, Hq, Hkv, T, D = 2, 16, 4, 8192, 128
+    k, v, q = rn(1, B, Hkv, T, D, dtype=BF16), rn(2, B, Hkv, T, D, dtype=BF16), rn(3, B, Hq, 1, D, dtype=BF16)
+    lens = torch.tensor([8192, 777], dtype=torch.int32, device=DEV)
+    kd, vd, qd = (t.to(DEV).transpose(1, 2) for t in (k, v, q))
+    want = tokens.attention(qd.contiguous(), kd.contiguous(), vd.contiguous(), k_len=lens, causal=True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = tokens.attention(qd, kd, vd, k_len=lens, causal=True)
+    assert torch.cuda.max_memory_allocated() - before < k.numel() * 2 // 4
+    assert torch.equal(got, want)
+    one = R.attention(q[1:].transpose(1, 2), k[1:, :, :777].transpose(1, 2), v[1:, :, :777].transpose(1, 2))["o"]
+    R.within(got[1:], one, "o")
+    leaves = [t.detach().requires_grad_(True) for t in (qd[:, :, :4], kd[:, :, :1], vd[:, :, :1])]      # gradients in the same layout
+    tokens.attention(*leaves, k_len=lens).sum().backward()
+    dense = [t.detach().contiguous().requires_grad_(True) for t in leaves]
+    tokens.attention(*dense, k_len=lens).sum().backward()
+    assert all(torch.equal(a.grad, b.grad) for a, b in zip(leaves, dense))

@@ -346,7 +346,7 @@ int pdae_dropout_bwd(const void* dy, int64_t n, float p, uint64_t seed, uint64_t
  * an axis with one element is not looked at), fewer than 2^24 workgroups (tiles of 128 rows times heads and samples).  Sums, softmax statistics and partial
  * results fp32; bf16 tensors multiply in bf16 (probabilities and their gradients rounded to bf16 for the second product), fp32 tensors in three exact bf16
  * planes x six products
- * (an infinite element counts as NaN).  Results are the same bits every run.
+ * (an infinite element counts as NaN).  Any finite v gives a finite o (up to 2^20 keys).  Results are the same bits every run.
  * lse [B][Hq][Tq] (natural log) may be NULL in the forward; the backward needs it and o.  ws: pdae_mha_workspace_bytes(d, backward),
  * enough for calls with and without lengths. */
 typedef struct pdae_mha_desc {

@@ -24,7 +24,17 @@ typedef __attribute__((address_space(3))) mh_s16x4* mh_lds4;
 #define MH_LOG2E 1.4426950408889634f
 #define MH_LN2 0.6931471805599453f
 #define MH_INF __builtin_inff()
-#define MH_GROW 1073741824.f           // 2^30: how far a tile's weights may outgrow the running reference before it is moved
+// Range of the unnormalised output.  Weights are kept 2^-32 of what the running maximum would give them, and the reference moves when a lane's weights of
+// one tile (32 keys of 64, or 16 of 32) sum to more than MH_GROW: all weights of a row sum to less than keys x 2^-20, so sum p v stays below max |v| for up
+// to 2^20 keys, whatever finite v is; weights below 2^-94 of the row's largest are zero (fp32 and bf16 share their exponent range).  bf16: the
+// reference itself lies MH_LIFT above the maximum, which costs nothing in the loop; an exponent of -32 is exact to 2^-19, far below a bf16 weight's rounding.
+// fp32 keeps its exponents small and multiplies the weights.
+#define MH_LIFT 32.f
+#define MH_DOWN 2.3283064365386963e-10f      // 2^-32
+#define MH_GROW 1.52587890625e-5f      // 2^-16
+template <int NP> __device__ __forceinline__ float mh_lift() { return NP == 1 ? MH_LIFT : 0.f; }
+// natural log-sum-exp of a row from its reference and its sum of weights
+template <int NP> __device__ __forceinline__ float mh_lse(float m, float l) { return ((m - mh_lift<NP>()) + __builtin_amdgcn_logf(l * (1.f / MH_DOWN))) * MH_LN2; }
 template <int I> struct MhInt { static constexpr int value = I; };
 
 struct MhaParams {

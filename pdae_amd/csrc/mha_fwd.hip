@@ -4,7 +4,7 @@
 // buffered: the next tile is on its way while this one is multiplied (bf16 with D a multiple of 8: straight into LDS, else through registers), one barrier a
 // tile.  Per 32 keys x 32 queries: S^T = K Q^T (DP / 16 MFMAs), p = 2^(sc2 s - reference), O^T += V^T P (DP / 16 MFMAs).
 // Every lane holds 16 of a column's 32 scores: the row maximum is a register tree and one exchange with lane ^ 32, the sum stays per lane until the end.
-// The reference is the maximum when it is set, and only moves when a tile's weights outgrow it by MH_GROW: then the accumulators are scaled, else nothing is.
+// The reference is the maximum (bf16: MH_LIFT above it) when it is set, and only moves when a tile's weights outgrow MH_GROW: then the accumulators are scaled.
 //
 // Bound: the matrix cores at the chip's power limit.  4 x 16 heads of 128, 4096 tokens, causal, bf16: 302 us (910 TFLOP/s; the library's 8192^3 product runs at
 // 1320), clock 1.63 GHz of 2.4, matrix pipes busy 54 % of the CUs' time, vector instructions 45 %, LDS 27 %, no bank conflicts.  4 x 8 heads of 64, 4096 tokens: 145 us
@@ -76,7 +76,11 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
       for (int s = 0; s < 2; ++s) {
         float e[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][s * 8 + j], P.sc2, -ref)); sum += e[j]; }
+        for (int j = 0; j < 8; ++j) {
+          e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][s * 8 + j], P.sc2, -ref));
+          if (NP == 3) e[j] *= MH_DOWN;
+          sum += e[j];
+        }
         mh_planes<NP>(e, F[kb][s]);
       }
     return sum;
@@ -121,8 +125,8 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) mh_mask_keys(S[a][kb], k0 + kb * 32 + 4 * h, kmax[a]);
         }
-        // p = 2^(t - ms) with the reference ms of the tiles before: fp32 and bf16 share their exponent range, so ms only has to be NEAR the maximum.  It
-        // moves (below) when a column has seen no key yet or a tile outgrows it by MH_GROW, which leaves three instructions a score here.
+        // p = 2^(t - ms) with the reference ms of the tiles before, which only has to be NEAR the maximum (MH_LIFT, MH_GROW: neither the weights nor their
+        // products with v leave the range).  It moves (below) when a column has seen no key yet or a tile outgrows it, which leaves three instructions a score here.
         float sum = weights(S[a], ms[a], F[a]);
         if (__any(m[a] == -MH_INF || !(sum <= MH_GROW))) {
           float mx = S[a][0][0];
@@ -131,7 +135,7 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[a][kb][r]);
           mx = fmaxf(mx, __shfl_xor(mx, 32));
-          const float mn = fmaxf(m[a], mx * P.sc2);
+          const float mn = fmaxf(m[a], __builtin_fmaf(mx, P.sc2, mh_lift<NP>()));
           ms[a] = mn == -MH_INF ? 0.f : mn;                                    // a column that has seen no key yet keeps p = 2^-inf = 0
           const float al = __builtin_amdgcn_exp2f(m[a] - ms[a]);
           m[a] = mn;
@@ -198,7 +202,7 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
         const float x2 = any ? O[a][d][g * 4 + 2] * inv : 0.f, x3 = any ? O[a][d][g * 4 + 3] * inv : 0.f;
         mh_store4<T, WH>(orow, d * 32 + g * 8 + he * 4, P.D, x0, x1, x2, x3);
       }
-    if (P.lse && he == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = any ? (m[a] + __builtin_amdgcn_logf(ls)) * MH_LN2 : -MH_INF;      // (v_log_f32: log2)
+    if (P.lse && he == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = any ? mh_lse<NP>(m[a], ls) : -MH_INF;      // (v_log_f32: log2)
   }
 }
 
@@ -260,8 +264,8 @@ __global__ void __launch_bounds__(256, OCC) mha_token_kernel(const MhaParams P) 
     float mx = S[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, S[r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32)) * P.sc2;
-    if (__any(m == -MH_INF || !(mx - m <= 30.f))) {                             // the reference only has to be near the maximum (see above)
+    mx = __builtin_fmaf(fmaxf(mx, __shfl_xor(mx, 32)), P.sc2, MH_LIFT);
+    if (__any(m == -MH_INF || !(mx - m <= 12.f))) {                             // weights up to 2^(12 - MH_LIFT) = 2^-20: the bound of MH_GROW
       const float mn = fmaxf(m, mx), msn = mn == -MH_INF ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - msn);
       m = mn; ms = msn; l *= al;
 #pragma unroll
@@ -330,7 +334,7 @@ __global__ void __launch_bounds__(256, OCC) mha_token_kernel(const MhaParams P) 
     const int tr = r / P.GP, hr = hp * P.GP + r % P.GP;
     tk_bf16* orow = (tk_bf16*)P.out + b * P.ob + (long long)tr * P.ot + (long long)hr * P.oh;
     mh_store4<tk_bf16, true>(orow, c, P.D, L != 0.f ? o[0] * inv : 0.f, L != 0.f ? o[1] * inv : 0.f, L != 0.f ? o[2] * inv : 0.f, L != 0.f ? o[3] * inv : 0.f);
-    if (P.lse && c == 0) P.lse[((long long)b * P.Hq + hr) * P.Tq + tr] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * MH_LN2 : -MH_INF;
+    if (P.lse && c == 0) P.lse[((long long)b * P.Hq + hr) * P.Tq + tr] = L != 0.f ? mh_lse<1>(M, L) : -MH_INF;
   }
 }
 
@@ -368,7 +372,7 @@ __global__ void __launch_bounds__(256) mha_join_kernel(const MhaParams P) {
   T* orow = (T*)P.out + b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh;
   if constexpr (V == 4) mh_store4<T, true>(orow, c, P.D, L != 0.f ? o[0] * inv : 0.f, L != 0.f ? o[1] * inv : 0.f, L != 0.f ? o[2] * inv : 0.f, L != 0.f ? o[3] * inv : 0.f);
   else TkVec<T>::store(orow + c, L != 0.f ? o[0] * inv : 0.f);
-  if (P.lse && c == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = L != 0.f ? (M + __builtin_amdgcn_logf(L)) * MH_LN2 : -MH_INF;
+  if (P.lse && c == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = L != 0.f ? mh_lse<MhNP<T>::NP>(M, L) : -MH_INF;
 }
 // The same for few rows in many ranges: a block per row, its G = 256 / lanes groups take every G-th range and are added in group order through LDS (one
 // thread after another through 32 ranges of a single token was 19 us of latency beside 7 us of attention).
@@ -409,7 +413,7 @@ __global__ void __launch_bounds__(256) mha_join_row_kernel(const MhaParams P) {
   for (int k = 0; k < 8; ++k) { x += wsum[k][t]; l += wsum[k][128]; }
   const int unit = (int)(i / P.R), r = (int)(i % P.R), b = unit / P.HP, hq = unit % P.HP * P.GP + r % P.GP, tq = r / P.GP;
   TkVec<T>::store((T*)P.out + b * P.ob + (long long)tq * P.ot + (long long)hq * P.oh + t, l != 0.f ? x / l : 0.f);
-  if (P.lse && t == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = l != 0.f ? (M + __builtin_amdgcn_logf(l)) * MH_LN2 : -MH_INF;
+  if (P.lse && t == 0) P.lse[((long long)b * P.Hq + hq) * P.Tq + tq] = l != 0.f ? mh_lse<MhNP<T>::NP>(M, l) : -MH_INF;
 }
 template <typename T> static void mh_join(const MhaParams& P, hipStream_t st) {
   if (P.splits >= 4 && P.splits <= 256 && (long long)P.units * P.R <= 4096) {

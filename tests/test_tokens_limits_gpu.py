@@ -83,3 +83,24 @@ def test_head_major_caches_are_read_in_place():
     dense = [t.detach().contiguous().requires_grad_(True) for t in leaves]
     tokens.attention(*dense, k_len=lens).sum().backward()
     assert all(torch.equal(a.grad, b.grad) for a, b in zip(leaves, dense))
+
+
+@pytest.mark.parametrize("B,Tq,Tk,Hq,Hkv,D,dtype", [(2, 40, 300, 2, 1, 32, F32), (1, 70, 300, 1, 1, 21, F32), (2, 200, 300, 2, 2, 128, BF16), (1, 150, 300, 1, 1, 13, BF16),
+                                                    (4, 256, 300, 64, 64, 32, BF16), (2, 1, 300, 8, 2, 64, BF16), (1, 1, 6000, 4, 1, 128, BF16), (1, 3, 6000, 2, 1, 64, F32)])
+def test_values_near_the_types_largest_while_the_scores_grow(B, Tq, Tk, Hq, Hkv, D, dtype):
+    """Scores rise by 20 (29 powers of two) from the first key tile to the last and the values are 1e37 .. 3e38: the weights sum to one, so every output
+    is finite, whatever reference the running sums are kept against."""
+    from pdae_amd import tokens
+    q, k = rn(1, B, Tq, Hq, D, scale=0.1), rn(2, B, Tk, Hkv, D, scale=0.1)
+    q[..., 0], k[..., 0] = 4.0, (torch.arange(Tk) * (5.0 / Tk))[None, :, None]
+    v = rn(3, B, Tk, Hkv, D).clamp(-3, 3) * 1e38
+    g = rn(4, B, Tq, Hq, D, scale=1e-20)
+    q, k, v, g = (t.to(dtype) for t in (q, k, v, g))
+    assert torch.isfinite(v.float()).all()
+    ref = R.attention(q, k, v, scale=1.0, d_o=g)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    o = tokens.attention(*leaves, scale=1.0)
+    o.backward(g.to(DEV))
+    R.within(o, ref["o"], "o")
+    for name, t in zip(("dq", "dk", "dv"), leaves):
+        R.within(t.grad, ref[name], name)

@@ -33,6 +33,12 @@ typedef __attribute__((address_space(3))) mh_s16x4* mh_lds4;
 #define MH_DOWN 2.3283064365386963e-10f      // 2^-32
 #define MH_GROW 1.52587890625e-5f      // 2^-16
 template <int NP> __device__ __forceinline__ float mh_lift() { return NP == 1 ? MH_LIFT : 0.f; }
+// the reference that a row maximum asks for.  (Not contracted: the fused form keeps MH_LIFT in a vector register, one too many where a wave has 64 rows.)
+template <int NP> __device__ __forceinline__ float mh_reference(float mx, float sc2) {
+#pragma clang fp contract(off)
+  const float t = mx * sc2;
+  return NP == 1 ? t + MH_LIFT : t;
+}
 // natural log-sum-exp of a row from its reference and its sum of weights
 template <int NP> __device__ __forceinline__ float mh_lse(float m, float l) { return ((m - mh_lift<NP>()) + __builtin_amdgcn_logf(l * (1.f / MH_DOWN))) * MH_LN2; }
 template <int I> struct MhInt { static constexpr int value = I; };

@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, S[a][kb][r]);
           mx = fmaxf(mx, __shfl_xor(mx, 32));
-          const float mn = fmaxf(m[a], __builtin_fmaf(mx, P.sc2, mh_lift<NP>()));
+          const float mn = fmaxf(m[a], mh_reference<NP>(mx, P.sc2));
           ms[a] = mn == -MH_INF ? 0.f : mn;                                    // a column that has seen no key yet keeps p = 2^-inf = 0
           const float al = __builtin_amdgcn_exp2f(m[a] - ms[a]);
           m[a] = mn;
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(256, OCC) mha_token_kernel(const MhaParams P) 
     float mx = S[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, S[r]);
-    mx = __builtin_fmaf(fmaxf(mx, __shfl_xor(mx, 32)), P.sc2, MH_LIFT);
+    mx = mh_reference<1>(fmaxf(mx, __shfl_xor(mx, 32)), P.sc2);
     if (__any(m == -MH_INF || !(mx - m <= 12.f))) {                             // weights up to 2^(12 - MH_LIFT) = 2^-20: the bound of MH_GROW
       const float mn = fmaxf(m, mx), msn = mn == -MH_INF ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - msn);
       m = mn; ms = msn; l *= al;

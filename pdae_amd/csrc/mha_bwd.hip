@@ -447,9 +447,19 @@ int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   P.part = (float*)ws + L.delta_floats;
   const long long nq = (long long)P.B * P.Hq * P.Tq, nk = (long long)P.B * P.Hkv * P.Tk;
   PDAE_CHECK_ARG(nq * P.D / 256 < (1ll << 31) && nk * P.D / 256 < (1ll << 31), "mha_bwd: too many rows for one launch");
+  const auto query_side = [&] { P.units = P.B * P.Hq; P.tiles = L.dq_tiles; P.splits = L.dq_splits; };
+  const auto key_side = [&] { P.units = P.B * P.Hkv; P.tiles = L.dkv_tiles; P.splits = L.dkv_splits; };
+  // every check stands before the first launch: a refused call has written nothing
   if (P.Tq > 0) {
-    P.units = P.B * P.Hq; P.tiles = L.dq_tiles; P.splits = L.dq_splits;
+    query_side();
     PDAE_CHECK_ARG(mh_grid(P) < (1 << 24), "mha_bwd: too many query tiles for one launch");
+  }
+  if (P.Tk > 0) {
+    key_side();
+    PDAE_CHECK_ARG(mh_grid(P) < (1 << 24) && (long long)cdiv(P.Tq, 32) * P.G < (1ll << 31), "mha_bwd: too many tiles for one launch");
+  }
+  if (P.Tq > 0) {
+    query_side();
     if (bf) {
       if (P.D & 7) mh_dq_go<tk_bf16, 128, 64, 1, false>(P, st);
       else if (P.D <= 32) mh_dq_go<tk_bf16, 32, 64, 2>(P, st);
@@ -470,8 +480,7 @@ int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
     }
   }
   if (P.Tk > 0) {
-    P.units = P.B * P.Hkv; P.tiles = L.dkv_tiles; P.splits = L.dkv_splits;
-    PDAE_CHECK_ARG(mh_grid(P) < (1 << 24) && (long long)cdiv(P.Tq, 32) * P.G < (1ll << 31), "mha_bwd: too many tiles for one launch");
+    key_side();
     if (bf) {
       if (P.D & 7) mh_dkv_go<tk_bf16, 128, 32, 1, false>(P, st);
       else if (P.D <= 32) mh_dkv_go<tk_bf16, 32, 32, 2>(P, st);

@@ -475,6 +475,7 @@ int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   const size_t need = mh_fwd_part_floats(P) * sizeof(float);
   PDAE_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "mha_fwd: needs %zu bytes of workspace (got %zu)", need, ws ? ws_bytes : (size_t)0);
   PDAE_CHECK_ARG(mh_grid(P) < (1 << 24) && (long long)P.units * P.R < (1ll << 31), "mha_fwd: too many query rows for one launch");
+  PDAE_CHECK_ARG(P.splits == 1 || (long long)P.units * P.R * P.D / 256 < (1ll << 31), "mha_fwd: too many query rows for one launch");      // (the join)
   P.part = (float*)ws;
   const int qb = mh_qb(P, dtype);
   if (mh_token(P, dtype)) {
@@ -497,7 +498,6 @@ int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   }
   if (int e = pdae_launch_status("mha_fwd")) return e;
   if (P.splits > 1) {
-    PDAE_CHECK_ARG((long long)P.units * P.R * P.D / 256 < (1ll << 31), "mha_fwd: too many query rows for one launch");
     if (dtype == PDAE_DT_BF16) mh_join<tk_bf16>(P, st);
     else mh_join<float>(P, st);
     return pdae_launch_status("mha_join");

@@ -35,3 +35,10 @@ def test_strides_of_one_element_axes_are_not_looked_at(H):
         refuses(H, H.op_mha_fwd(H.Mha(1, 2, 2, 2, 2, 8, **{k + "_stride": s}), P, P, P, P), "token stride")
     refuses(H, H.op_mha_fwd(H.Mha(2, 1, 1, 1, 1, 8, v_stride=(far, 1, 1)), P, P, P, P), "out of range")
     refuses(H, H.op_mha_fwd(H.Mha(1, 1, 4, 2, 1, 8, q_stride=(1, 1, 1 << 27)), P, P, P, P), "head stride")
+
+
+def test_attention_is_refused_before_anything_is_launched(H):
+    """Every size check stands in front of the first launch: a refused backward has not written dq or the workspace.  (Here a launch ends in another error.)"""
+    a = H.Mha(1, 1, (1 << 30) - 1, 2, 2, 8)                                # 2^23 key tiles of two heads
+    bwd = H.op_mha_bwd(a, P, P, P, P, P, P, P, P, P, ws=P, ws_bytes=1 << 60)
+    refuses(H, bwd, "too many")

@@ -458,6 +458,14 @@ int k_mha_bwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
     key_side();
     PDAE_CHECK_ARG(mh_grid(P) < (1 << 24) && (long long)cdiv(P.Tq, 32) * P.G < (1ll << 31), "mha_bwd: too many tiles for one launch");
   }
+  const void* in[5] = {P.Tq ? P.q : nullptr, P.Tk ? P.k : nullptr, P.Tk ? P.v : nullptr, P.Tq ? P.o : nullptr, P.Tq ? P.d_o : nullptr};
+  const void* out[3] = {P.Tq ? P.dq : nullptr, P.Tk ? P.dk : nullptr, P.Tk ? P.dv : nullptr};
+  for (int i = 0; i < 3; ++i) {
+    bool own = true;
+    for (const void* x : in) own = own && (!out[i] || out[i] != x);
+    for (int j = 0; j < i; ++j) own = own && (!out[i] || out[i] != out[j]);
+    PDAE_CHECK_ARG(own, "mha_bwd: a gradient in the place of an input or of another gradient");
+  }
   if (P.Tq > 0) {
     query_side();
     if (bf) {

@@ -476,6 +476,7 @@ int k_mha_fwd(const MhaParams& P0, int dtype, void* ws, size_t ws_bytes, hipStre
   PDAE_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "mha_fwd: needs %zu bytes of workspace (got %zu)", need, ws ? ws_bytes : (size_t)0);
   PDAE_CHECK_ARG(mh_grid(P) < (1 << 24) && (long long)P.units * P.R < (1ll << 31), "mha_fwd: too many query rows for one launch");
   PDAE_CHECK_ARG(P.splits == 1 || (long long)P.units * P.R * P.D / 256 < (1ll << 31), "mha_fwd: too many query rows for one launch");      // (the join)
+  PDAE_CHECK_ARG(P.out != P.q && (P.Tk == 0 || (P.out != P.k && P.out != P.v)), "mha_fwd: o in the place of q, k or v");
   P.part = (float*)ws;
   const int qb = mh_qb(P, dtype);
   if (mh_token(P, dtype)) {

@@ -42,3 +42,22 @@ def test_attention_is_refused_before_anything_is_launched(H):
     a = H.Mha(1, 1, (1 << 30) - 1, 2, 2, 8)                                # 2^23 key tiles of two heads
     bwd = H.op_mha_bwd(a, P, P, P, P, P, P, P, P, P, ws=P, ws_bytes=1 << 60)
     refuses(H, bwd, "too many")
+
+
+def test_gradients_in_the_place_of_what_is_still_read_are_refused(H):
+    """Layer norm up to 1024 rows: blocks of columns read x and dy beside the blocks that write dx, and attention's second kernel reads what the first has written
+    over -- in place they gave wrong weight gradients without a word."""
+    W, Q = 1 << 20, P + 4096
+    bwd = lambda x, dy, dx, add=None: H.op_layernorm_bwd(x, P, P, P, dy, 4, 8, dx, P, P, P, ws_bytes=1 << 20, add=add)
+    refuses(H, bwd(P, Q, P), "in the place of")
+    refuses(H, bwd(P, Q, Q), "in the place of")
+    refuses(H, bwd(P, Q, Q, add=Q), "in the place of")
+    a = H.Mha(2, 4, 4, 2, 2, 8)
+    p = [P + 4096 * i for i in range(9)]
+    for i in range(3):
+        refuses(H, H.op_mha_fwd(a, *p[:3], p[i]), "in the place of")
+    for out in range(3):
+        for other in [0, 1, 2, 3, 5] + [6 + j for j in range(3) if j != out]:
+            t = list(p)
+            t[6 + out] = p[other]
+            refuses(H, H.op_mha_bwd(a, *t, ws=P + W, ws_bytes=1 << 30), "in the place of")

@@ -318,7 +318,7 @@ int pdae_attn_bwd(const float* qkv, const float* out, const float* lse, const fl
 
 /* y = (x - mu) rstd gamma + beta per row of C channels (biased variance, rstd = 1 / sqrt(var + eps)); next to pdae_mlp_modln_* (which fuses the
  * condition scale and SiLU of MLPSkipNet, fp32 only) this is the bare norm.  ldx / ldy: row strides in elements (>= C);
- * C <= 2^24.  gamma, beta, mean, rstd may be NULL. */
+ * C <= 2^24.  gamma, beta, mean, rstd may be NULL.  y may be x (with ldy = ldx); no other output may overlap an input. */
 int pdae_layernorm_fwd(const void* x, int64_t ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, int64_t ldy, float* mean, float* rstd,
                        int dtype, pdae_stream_t stream);
 /* dx = LayerNorm backward (+ add, the identity path around the norm); dgamma / dbeta (+)= sums over the rows, in a fixed order (acc_param selects "+=";

@@ -29,9 +29,10 @@ template <int L> __device__ __forceinline__ float ln_sum(float v, float* red) {
 #define LN_THREADS(L) ((L) > 256 ? (L) : 256)
 
 // Elements of a row: nv = C / 8 whole vectors (vector i of lane `lane` is number lane + i * lanes) and C % 8 single elements on the first lanes.
+// y may be x: a lane writes the elements that it has read, after the row's sums (x and y are not declared apart).
 template <typename T, int L, int NV>
-__global__ void __launch_bounds__(LN_THREADS(L)) layernorm_fwd_kernel(const T* __restrict__ x, long long ldx, const float* __restrict__ gamma,
-                                                             const float* __restrict__ beta, int R, int C, float eps, T* __restrict__ y, long long ldy,
+__global__ void __launch_bounds__(LN_THREADS(L)) layernorm_fwd_kernel(const T* x, long long ldx, const float* __restrict__ gamma,
+                                                             const float* __restrict__ beta, int R, int C, float eps, T* y, long long ldy,
                                                              float* __restrict__ mean, float* __restrict__ rstd) {
   __shared__ float red[8];
   constexpr int RPB = LN_THREADS(L) / L;
@@ -465,6 +466,7 @@ int k_layernorm_fwd(const void* x, long long ldx, const float* gamma, const floa
   if (R == 0) return PDAE_OK;
   PDAE_CHECK_ARG(x && y, "layernorm_fwd: null pointer");
   PDAE_CHECK_ARG(tk_aligned(x, dtype) && tk_aligned(y, dtype), "layernorm: tensors must be aligned to their element size");
+  PDAE_CHECK_ARG(y != x || ldy == ldx, "layernorm_fwd: y in the place of x with another row stride");
   if (dtype == PDAE_DT_F32) ln_fwd<float>(x, ldx, gamma, beta, R, C, eps, y, ldy, mean, rstd, st);
   else ln_fwd<tk_bf16>(x, ldx, gamma, beta, R, C, eps, y, ldy, mean, rstd, st);
   return pdae_launch_status("layernorm_fwd");

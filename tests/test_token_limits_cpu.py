@@ -48,6 +48,7 @@ def test_gradients_in_the_place_of_what_is_still_read_are_refused(H):
     """Layer norm up to 1024 rows: blocks of columns read x and dy beside the blocks that write dx, and attention's second kernel reads what the first has written
     over -- in place they gave wrong weight gradients without a word."""
     W, Q = 1 << 20, P + 4096
+    refuses(H, H.op_layernorm_fwd(P, P, P, 4, 8, 1e-5, P, ldx=8, ldy=9), "in the place of")      # (with one stride it is allowed)
     bwd = lambda x, dy, dx, add=None: H.op_layernorm_bwd(x, P, P, P, dy, 4, 8, dx, P, P, P, ws_bytes=1 << 20, add=add)
     refuses(H, bwd(P, Q, P), "in the place of")
     refuses(H, bwd(P, Q, Q), "in the place of")

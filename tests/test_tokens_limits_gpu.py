@@ -104,3 +104,18 @@ def test_values_near_the_types_largest_while_the_scores_grow(B, Tq, Tk, Hq, Hkv,
     R.within(o, ref["o"], "o")
     for name, t in zip(("dq", "dk", "dv"), leaves):
         R.within(t.grad, ref[name], name)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,C", [(300, 64), (1100, 71), (33, 520), (1500, 1536), (5, 4099), (7, 16384), (5, 16391), (3, 40000)])
+def test_layer_norm_in_place_is_the_same_bits(rows, C, dtype):
+    from pdae_amd import hip as H
+    k = H.DTYPES[dtype]
+    x = rn(1, rows, C + 5, dtype=dtype).to(DEV)
+    g, b = rn(2, C).to(DEV), rn(3, C).to(DEV)
+    y, m, r = torch.empty_like(x), torch.empty(rows, device=DEV), torch.empty(rows, device=DEV)
+    y.copy_(x)
+    H.run(H.op_layernorm_fwd(x, g, b, rows, C, 1e-5, y, m, r, dtype=k, ldx=C + 5, ldy=C + 5))
+    R.within(y[:, :C], R.layer_norm(x[:, :C].cpu(), g.cpu(), b.cpu(), 1e-5)["y"], "y")
+    H.run(H.op_layernorm_fwd(x, g, b, rows, C, 1e-5, x, dtype=k, ldx=C + 5, ldy=C + 5))
+    assert torch.equal(x, y)                                    # what lies between the rows included

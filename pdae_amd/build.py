@@ -32,6 +32,15 @@ def _newer(src_list, target):
     return any(os.path.getmtime(s) > tt for s in src_list)
 
 
+def _made_with(obj):
+    """Flags that an object was compiled with (kept beside it), or None."""
+    try:
+        with open(obj + ".flags") as f:
+            return f.read()
+    except OSError:
+        return None
+
+
 def _hazard_scan(src):
     """The device assembly hipcc left next to the object (--save-temps=obj) must be free of both store-operand hazard patterns; all temporaries
     are removed afterwards."""
@@ -63,17 +72,23 @@ def build_library(force=False, verbose=True):
         src = os.path.join(CSRC, s)
         obj = os.path.join(LIBDIR, s.replace(".hip", ".o"))
         objs.append(obj)
-        if force or _newer([src] + hdrs, obj):
-            cmd = [HIPCC] + FLAGS + EXTRA_FLAGS.get(s, []) + (["--save-temps=obj"] if s in HAZARD_SCAN else []) + ["-c", src, "-o", obj]
+        cmd = [HIPCC] + FLAGS + EXTRA_FLAGS.get(s, []) + (["--save-temps=obj"] if s in HAZARD_SCAN else [])
+        flags = " ".join(cmd)
+        if force or _made_with(obj) != flags or _newer([src] + hdrs, obj):
+            cmd += ["-c", src, "-o", obj]
             if verbose:
                 print(" ".join(cmd), flush=True)
-            procs.append((s, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
-    for s, p in procs:
+            if os.path.exists(obj + ".flags"):
+                os.remove(obj + ".flags")                      # written again when the object is whole
+            procs.append((s, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT), obj, flags))
+    for s, p, obj, flags in procs:
         out, _ = p.communicate()
         if p.returncode != 0:
             raise RuntimeError(f"hipcc failed on {s}:\n{out.decode()}")
         if s in HAZARD_SCAN:
             _hazard_scan(s)
+        with open(obj + ".flags", "w") as f:
+            f.write(flags)
     if force or procs or _newer(objs, LIB):
         cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs + ["-ldl"]
         if verbose:

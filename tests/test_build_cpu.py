@@ -40,3 +40,12 @@ def test_changed_flags_compile_an_object_anew(sandbox):
     assert build() == ["a.hip", "link"]
     os.utime(os.path.join(B.CSRC, "a.hip"), (2 ** 31 - 1,) * 2)
     assert build() == ["a.hip", "link"]
+
+
+def test_the_entry_point_compiles_every_source_every_time(monkeypatch):
+    import __graft_entry__ as entry
+    from pdae_amd import build as B
+    asked = []
+    monkeypatch.setattr(B, "build_library", lambda **k: asked.append(k) or B.LIB)
+    entry.build()
+    assert asked == [dict(force=True, verbose=True)]

@@ -73,6 +73,7 @@ class PdaeError(RuntimeError):
 
 
 _lib = None
+ABI_VERSION = 11            # pdae_abi_version() of include/pdae_hip.h
 
 
 def lib():
@@ -83,6 +84,13 @@ def lib():
             raise PdaeError(f"{LIB_PATH} is missing -- run `python -m pdae_amd.build` (hipcc, gfx950). "
                             "pdae_amd has no CPU fallback.")
         L = ctypes.CDLL(LIB_PATH)
+        # the number alone does not tell: entry points may be added under it
+        L.pdae_abi_version.restype = ctypes.c_int
+        if L.pdae_abi_version() != ABI_VERSION:
+            raise PdaeError(f"{LIB_PATH} has ABI {L.pdae_abi_version()}, this package needs {ABI_VERSION} -- run `python -m pdae_amd.build`")
+        lacks = [n for n in EXPORTS if not hasattr(L, n)]
+        if lacks:
+            raise PdaeError(f"{LIB_PATH} is older than this package: it lacks {', '.join(lacks[:4])}{' ...' if len(lacks) > 4 else ''} -- run `python -m pdae_amd.build`")
         L.pdae_last_error.restype = ctypes.c_char_p
         L.pdae_run_ops.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
         L.pdae_run_ops.restype = ctypes.c_int
@@ -95,7 +103,6 @@ def lib():
         L.pdae_gn_workspace_bytes.restype = ctypes.c_size_t
         L.pdae_colsum_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int]
         L.pdae_colsum_workspace_bytes.restype = ctypes.c_size_t
-        L.pdae_abi_version.restype = ctypes.c_int
         L.pdae_conv_gnbwd_bytes.argtypes = [ctypes.POINTER(ConvDesc), ctypes.c_int, ctypes.c_void_p]
         L.pdae_conv_gnbwd_bytes.restype = ctypes.c_size_t
         L.pdae_conv_stats_bytes.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]

@@ -62,3 +62,18 @@ def test_gradients_in_the_place_of_what_is_still_read_are_refused(H):
             t = list(p)
             t[6 + out] = p[other]
             refuses(H, H.op_mha_bwd(a, *t, ws=P + W, ws_bytes=1 << 30), "in the place of")
+
+
+@pytest.mark.parametrize("version,says", [(11, "lacks pdae_"), (10, "ABI 10")])
+def test_an_older_library_is_named_as_such(tmp_path, version, says):
+    """Entry points were added without a new ABI number: a library of the number that lacks them is refused with what it lacks, not with an AttributeError later."""
+    import os
+    import subprocess
+    import sys
+    src, so = tmp_path / "old.c", tmp_path / "old.so"
+    names = ["pdae_run_ops", "pdae_conv2d_wgrad_workspace_bytes", "pdae_gn_workspace_bytes"]
+    src.write_text('const char* pdae_last_error(void) { return ""; }\nint pdae_abi_version(void) { return %d; }\n' % version + "".join(f"int {n}(void) {{ return 0; }}\n" for n in names))
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(so), str(src)], check=True)
+    r = subprocess.run([sys.executable, "-c", "from pdae_amd import hip\ntry:\n    hip.lib()\nexcept hip.PdaeError as e:\n    print('refused:', e)"], capture_output=True, text=True,
+                       env=dict(os.environ, PDAE_HIP_LIB=str(so)), cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and r.stdout.startswith("refused:") and says in r.stdout and str(so) in r.stdout, r.stdout + r.stderr[-600:]

@@ -413,7 +413,7 @@ enum {
    * seed, step, layer;  DROPOUT_BWD + accumulate;  MHA_* the eight int32 of the descriptor, its twelve strides, ws_bytes (f[0] = scale) */
   PDAE_OP_LAYERNORM_FWD, PDAE_OP_LAYERNORM_BWD, PDAE_OP_DROPOUT_FWD, PDAE_OP_DROPOUT_BWD, PDAE_OP_MHA_FWD, PDAE_OP_MHA_BWD
 };
-/* pdae_op.flags (ABI 10; the field was `reserved`, always 0).  PDAE_OPF_SIDE: issue this op on the executor's second (low-priority) stream.
+/* pdae_op.flags (ABI 10; the field was `reserved`, always 0).  PDAE_OPF_SIDE: issue this op on the executor's second stream (of the default priority).
  * It starts when the ops in front of it in the array have finished, and runs beside the ops behind it until the next PDAE_OP_JOIN or the end
  * of the pdae_run_ops call (which joins).  The caller guarantees that no op between a side op and the next join overwrites the side op's
  * inputs or touches its outputs.  Knob PDAE_SIDE_STREAM=0: the flag is ignored (everything in order on the caller's stream). */

@@ -667,7 +667,7 @@ class Mha:
     def __init__(self, B, Tq, Tk, Hq, Hkv, D, dtype=DT_F32, causal=False, scale=None, q_stride=None, k_stride=None, v_stride=None, o_stride=None):
         self.B, self.Tq, self.Tk, self.Hq, self.Hkv, self.D = B, Tq, Tk, Hq, Hkv, D
         self.dtype, self.causal = dtype, bool(causal)
-        self.scale = 1.0 / D ** 0.5 if scale is None else float(scale)
+        self.scale = 1.0 / max(D, 1) ** 0.5 if scale is None else float(scale)
         q, k = (Tq * Hq * D, Hq * D, D), (Tk * Hkv * D, Hkv * D, D)
         self.q_stride, self.k_stride = tuple(q_stride or q), tuple(k_stride or k)
         self.v_stride, self.o_stride = tuple(v_stride or k), tuple(o_stride or q)

@@ -77,3 +77,8 @@ def test_an_older_library_is_named_as_such(tmp_path, version, says):
     r = subprocess.run([sys.executable, "-c", "from pdae_amd import hip\ntry:\n    hip.lib()\nexcept hip.PdaeError as e:\n    print('refused:', e)"], capture_output=True, text=True,
                        env=dict(os.environ, PDAE_HIP_LIB=str(so)), cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode == 0 and r.stdout.startswith("refused:") and says in r.stdout and str(so) in r.stdout, r.stdout + r.stderr[-600:]
+
+
+def test_no_channels_are_refused_by_name(H):
+    """The default scale of zero channels is no number: the refusal is the kernels' own, not a division by zero."""
+    refuses(H, H.op_mha_fwd(H.Mha(2, 4, 4, 2, 1, 0), P, P, P, P), "head width 0")

@@ -3,8 +3,12 @@
 //   o[q] = sum_j p[q][j] v[j],   p[q][j] = exp(scale q.k[j] - lse[q]),   lse[q] = log sum_j exp(scale q.k[j])      over the keys j that row q sees
 //   key j is seen by query i of sample b iff  j < k_len[b]  and (causal)  j <= i + k_len[b] - q_len[b];   queries i >= q_len[b] do not exist.
 //
-// Element formats: bf16 tensors are ONE bf16 plane (NP = 1); fp32 tensors are split exactly into THREE (8 + 8 + 8 mantissa bits) whose six leading products
-// are accumulated (NP = 3, ~2^-23 a product: fp32 grade, free of range limits).  Everything that is summed is fp32.
+// Element formats: bf16 tensors are ONE bf16 plane (NP = 1); fp32 tensors are split exactly into THREE (8 + 8 + 8 mantissa bits, by truncation) whose six
+// leading products are accumulated (NP = 3).  What is dropped of a product is below 2^-20 |a||b| (2 x 2^-7 x 2^-14), 2^-24.5 in the mean over normally
+// distributed values: the bound is sixteen times a rounding to fp32, the mean is one.  Below 2^-110 the lower planes leave fp32's range.  Everything that is
+// summed is fp32.
+// Roundings to fewer bits in bf16 tensors: the weights p (before p v and p^T dO) and dS (before dS K and dS^T Q) become bf16, because the matrix cores take
+// bf16: up to 2^-8 of each value, 1.7e-3 of the norm.  A caller who needs more has fp32 tensors.
 //
 // Fragments of v_mfma_f32_32x32x16_bf16: lane l gives A[row l%32][k (l/32)*8 ..+7] and B[k (l/32)*8 ..+7][col l%32]; accumulator register r is
 // D[(r&3) + 8*(r>>2) + 4*(l/32)][l%32].  The kernels always put the side whose statistics matter on the COLUMNS (queries in the forward and dQ

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256, OCC) mha_fwd_kernel(const MhaParams P) {
   bool live = false;
 #pragma unroll
   for (int a = 0; a < QB; ++a) {
-    const int r = row0 + wv * (32 * QB) + a * 32 + li, tq = r / P.GP, hq = hp * P.GP + r % P.GP;
+    const int r = row0 + wv * (32 * QB) + a * 32 + li, tq = r / P.GP;
     const bool ok = r < P.R && tq < lq;
     kmax[a] = ok ? (P.causal ? min(lk, tq + off + 1) : lk) : lk;               // rows that do not exist never force the masked path; they are zeroed at the end
     live = live || ok;
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(256, OCC) mha_token_kernel(const MhaParams P) 
   const tk_bf16* vbase = (const tk_bf16*)P.v + b * P.vb + hk * P.vh;
   const int nk = max(0, lq <= 0 ? 0 : P.causal ? min(lk, min((P.R - 1) / P.GP, lq - 1) + off + 1) : lk), ntiles = (nk + 31) / 32;
   const int tb = (int)((long long)ntiles * split / P.splits), te = (int)((long long)ntiles * (split + 1) / P.splits);
-  const int tq = li / P.GP, hq = hp * P.GP + li % P.GP;
+  const int tq = li / P.GP;
   const bool ok = li < P.R && tq < lq;
   const int kmax = ok ? (P.causal ? min(lk, tq + off + 1) : lk) : lk;
   mh_bf16x8 Q[KS][1];

@@ -26,14 +26,12 @@ __device__ __forceinline__ unsigned tk_pack2(float a, float b) {
 // (global memory takes them unaligned): rows of an odd length and views at odd offsets run on the same path as aligned ones.
 template <typename T> struct TkVec;
 template <> struct TkVec<float> {
-  static constexpr int BYTES = 4;
   __device__ static __forceinline__ void load8(const float* p, float (&v)[8]) { __builtin_memcpy(v, p, 32); }
   __device__ static __forceinline__ void store8(float* p, const float (&v)[8]) { __builtin_memcpy(p, v, 32); }
   __device__ static __forceinline__ float load(const float* p) { return *p; }
   __device__ static __forceinline__ void store(float* p, float v) { *p = v; }
 };
 template <> struct TkVec<tk_bf16> {
-  static constexpr int BYTES = 2;
   __device__ static __forceinline__ void load8(const tk_bf16* p, float (&v)[8]) {
     unsigned w[4];
     __builtin_memcpy(w, p, 16);

@@ -344,8 +344,8 @@ int pdae_dropout_bwd(const void* dy, int64_t n, float p, uint64_t seed, uint64_t
  * Strides in elements; channels are contiguous.  Gradients have their tensor's strides (d_o those of o, dq of q, dk of k, dv of v).
  * No output may overlap an input or another output.  Limits: D <= 128, Hq a multiple of Hkv, scale > 0, token strides below 2^21 elements (the stride of
  * an axis with one element is not looked at), fewer than 2^24 workgroups (tiles of 128 rows times heads and samples).  Sums, softmax statistics and partial
- * results fp32; bf16 tensors multiply in bf16 (probabilities and their gradients rounded to bf16 for the second product), fp32 tensors in three exact bf16
- * planes x six products
+ * results fp32; bf16 tensors multiply in bf16 (probabilities, and for dk their gradients, are rounded to bf16 for the second product; dq takes the gradients in
+ * two bf16 planes), fp32 tensors in three exact bf16 planes x six products
  * (an infinite element counts as NaN).  Any finite v gives a finite o (up to 2^20 keys).  Results are the same bits every run.
  * lse [B][Hq][Tq] (natural log) may be NULL in the forward; the backward needs it and o.  ws: pdae_mha_workspace_bytes(d, backward),
  * enough for calls with and without lengths. */

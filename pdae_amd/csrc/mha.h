@@ -7,8 +7,8 @@
 // leading products are accumulated (NP = 3).  What is dropped of a product is below 2^-20 |a||b| (2 x 2^-7 x 2^-14), 2^-24.5 in the mean over normally
 // distributed values: the bound is sixteen times a rounding to fp32, the mean is one.  Below 2^-110 the lower planes leave fp32's range.  Everything that is
 // summed is fp32.
-// Roundings to fewer bits in bf16 tensors: the weights p (before p v and p^T dO) and dS (before dS K and dS^T Q) become bf16, because the matrix cores take
-// bf16: up to 2^-8 of each value, 1.7e-3 of the norm.  A caller who needs more has fp32 tensors.
+// Roundings to fewer bits in bf16 tensors: the weights p (before p v and p^T dO) and dS (before dS^T Q; two planes before dS K) become bf16, because the matrix
+// cores take bf16: up to 2^-8 of each value, 1.7e-3 of the norm.  A caller who needs more has fp32 tensors.
 //
 // Fragments of v_mfma_f32_32x32x16_bf16: lane l gives A[row l%32][k (l/32)*8 ..+7] and B[k (l/32)*8 ..+7][col l%32]; accumulator register r is
 // D[(r&3) + 8*(r>>2) + 4*(l/32)][l%32].  The kernels always put the side whose statistics matter on the COLUMNS (queries in the forward and dQ
@@ -121,6 +121,18 @@ template <int NP> __device__ __forceinline__ void mh_planes(const float (&e)[8],
 #pragma unroll
     for (int p = 0; p < 3; ++p) { const tk_u32x4 v = {w[p][0], w[p][1], w[p][2], w[p][3]}; f[p] = __builtin_bit_cast(mh_bf16x8, v); }
   }
+}
+// the same with a second bf16 plane for what the first rounding left (2^-17 of the value remains)
+__device__ __forceinline__ void mh_planes2(const float (&e)[8], mh_bf16x8 (&f)[2]) {
+  unsigned w[2][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = e[2 * j], b = e[2 * j + 1];
+    w[0][j] = tk_pack2(a, b);
+    w[1][j] = tk_pack2(a - __uint_as_float(w[0][j] << 16), b - __uint_as_float(w[0][j] & 0xffff0000u));
+  }
+#pragma unroll
+  for (int p = 0; p < 2; ++p) { const tk_u32x4 v = {w[p][0], w[p][1], w[p][2], w[p][3]}; f[p] = __builtin_bit_cast(mh_bf16x8, v); }
 }
 template <int NP> __device__ __forceinline__ void mh_mma(const mh_bf16x8 (&A)[NP], const mh_bf16x8 (&B)[NP], mh_f32x16& acc) {
   if constexpr (NP == 3) {                   // small terms first

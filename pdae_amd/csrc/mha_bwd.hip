@@ -8,8 +8,10 @@
 // results are the same bits every run.  dK / dV of a key head sum over the query heads that share it inside the kernel.
 // Bound: the matrix cores at the chip's power limit.  4 x 16 heads of 128, 4096 tokens, causal, bf16: dQ 452 us (910 TFLOP/s), dK / dV 581 us (945), clock 1.63 GHz of
 // 2.4, matrix pipes busy 54 / 57 % of the CUs' time, vector instructions 50 / 35 %, LDS 27 / 43 %, no bank conflicts.  fp32, 8 x 4 heads of 64, 1024 tokens: 88 + 111 us.
-// bf16: dQ is off by 2.4e-3 .. 2.5e-3 of its norm where one rounding of the output costs 1.7e-3: dS is rounded for the second product (1.7e-3) and delta comes from the
-// rounded o (up to 0.9e-3); both add up in squares.  dS in two planes (a product more): 1.8e-3, but 61 -> 72 us in a training pass of 185 (7 padded samples).
+// Roundings of bf16 tensors: dQ takes dS in TWO bf16 planes (a matrix instruction more on the same fragment): it is off by 1.65e-3 .. 1.85e-3 of its norm, of which its
+// own rounding is 1.65e-3 and delta from the rounded o up to 0.9e-3, in squares.  With one plane it was 2.5e-3, one and a half times what rounding the result
+// costs; the second plane is 7 % of a long training pass (4 x 16 heads of 128, 4096 tokens, causal: 1230 -> 1315 us; 7 padded samples 183 -> 195).  dK and dV round dS
+// and P once (2.3e-3 .. 2.4e-3): a second plane finds no registers beside K, V and both accumulators.
 // Few tiles: the summed axis is split into ranges (grid `splits`), every range leaves an fp32 partial, mha_bwd_join_kernel adds them in order.
 // Row validity is decided where rows are staged: queries that do not exist or (causal) see no key come as zeros with lse = +inf, so P = 0 exactly and
 // non-finite values in them reach nothing.
@@ -32,7 +34,7 @@ template <typename T, int DB, bool WH> __device__ __forceinline__ void mh_put(co
 template <typename T, int DP, int KT, int OCC, bool WH>
 __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
   constexpr int NP = MhNP<T>::NP, KS = DP / 16, DB = DP / 32, KB = KT / 32;
-  constexpr int TE = MhTile<NP, KT, DP>::ELEMS, MM = NP == 3 ? 6 : 1, PD = NP == 3 ? 2 : 4;
+  constexpr int TE = MhTile<NP, KT, DP>::ELEMS, MM = NP == 3 ? 6 : 1, PD = NP == 3 ? 2 : 4, SP = NP == 3 ? 3 : 2;      // SP: planes of dS
   extern __shared__ __attribute__((aligned(16))) unsigned short mh_sm[];       // [2 buffers][K tile | V tile]
   int unit, tile, split;
   if (!mh_where(P, unit, tile, split)) return;
@@ -158,7 +160,7 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
         __builtin_amdgcn_sched_barrier(0);
         const int base = k0 + kb * 32 + 4 * h;
         const bool cut = __any(k0 + kb * 32 + 32 > kmax);
-        mh_bf16x8 F[2][NP];
+        mh_bf16x8 F[2][SP];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           float e[8];
@@ -169,7 +171,8 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
             e[j] = p * (E[r] - del);
             if (cut && base + (r & 3) + 8 * (r >> 2) >= kmax) e[j] = 0.f;
           }
-          mh_planes<NP>(e, F[s]);
+          if constexpr (NP == 1) mh_planes2(e, F[s]);
+          else mh_planes<NP>(e, F[s]);
         }
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -177,9 +180,14 @@ __global__ void __launch_bounds__(256, OCC) mha_dq_kernel(const MhaParams P) {
           for (int s = 0; s < 2; ++s) {
             mh_bf16x8 A[NP];
             mh_frag_cols<NP, KT, DP>(cur, kb * 32 + s * 16, d, lane, A);
-            mh_mma<NP>(A, F[s], dQ[d]);
+            if constexpr (NP == 1) {                                           // small terms first
+              dQ[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], F[s][1], dQ[d], 0, 0, 0);
+              dQ[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[0], F[s][0], dQ[d], 0, 0, 0);
+            } else {
+              mh_mma<NP>(A, F[s], dQ[d]);
+            }
           }
-        mh_order<2 * DB, PD, 2 * NP, MM>();
+        mh_order<2 * DB, PD, 2 * NP, NP == 1 ? 2 : MM>();
         __builtin_amdgcn_sched_barrier(0);
       }
     }

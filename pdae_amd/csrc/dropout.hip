@@ -7,7 +7,7 @@
 // Bound: HBM.  One call of ten rounds serves four elements and costs ten 32 x 32 -> 64-bit multiplies (v_mad_u64_u32, quarter rate) and twenty xors,
 // ~280 issue cycles per 256 elements and SIMD = 2.2e12 elements/s on the chip: above the rate at which HBM delivers bf16 pairs (4 bytes an element,
 // 1.5e12 /s).  Eight elements a thread and pass (16-byte accesses in bf16, 2 x 16 in fp32).  41 M bf16 elements: with a residual 47 us (5.2 TB/s), without 27 us
-// (6.1); a large copy moves 5.2.  128 x 2048 fp32: 2.8 us, a launch.
+// (6.1); a large copy moves 5.2.  128 x 2048 fp32: 2.5 us, a launch.
 #include "token.h"
 #include "kernels.h"
 

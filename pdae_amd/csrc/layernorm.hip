@@ -3,8 +3,9 @@
 //
 // Bound: HBM (forward one read and one write of the tensor, backward two reads and one write).  A row is read ONCE and lives in registers between its
 // reductions: L lanes share it (8 .. 64 of a wave, or a block of 256 / 512), NV vectors of eight elements a lane; only rows beyond 16384 channels are
-// streamed again from L2 (NV = 0).  65536 x 1536 bf16: forward 78 us, backward 134 us + 5 for the partial rows
-// (5.2 / 4.5 TB/s; a large copy on this chip moves 5.2).  128 x 2048 fp32: 3.6 + 3.8 us, two launches.
+// streamed again from L2 (NV = 0).  65536 x 1536 bf16: forward 75 us, backward 133 us + 5 for the partial rows
+// (5.3 / 4.6 TB/s; a large copy on this chip moves 5.2; first ten passes 77 and 135 .. 141).  128 x 2048 fp32: 3.6 + 3.8 us, two launches.  9001 x 1027 bf16 forward: 11 .. 12 us
+// (3.3 TB/s): 8192 rows are resident, one a wave, and the last 809 run alone.
 // The variance is taken from the deviations (two passes over registers), not from E[x^2] - E[x]^2, which loses what a large mean leaves.
 //
 // Weight gradients: every block walks a fixed set of rows and keeps sum dy xh / sum dy of its lanes' own channels in registers; it leaves ONE partial row per

@@ -6,11 +6,12 @@
 //
 // Two kernels recompute S and dP twice (7 products of 2 Tq Tk D instead of 5): dK / dV and dQ then each have ONE writer, so there are no atomics and the
 // results are the same bits every run.  dK / dV of a key head sum over the query heads that share it inside the kernel.
-// Bound: the matrix cores at the chip's power limit.  4 x 16 heads of 128, 4096 tokens, causal, bf16: dQ 452 us (910 TFLOP/s), dK / dV 581 us (945), clock 1.63 GHz of
-// 2.4, matrix pipes busy 54 / 57 % of the CUs' time, vector instructions 50 / 35 %, LDS 27 / 43 %, no bank conflicts.  fp32, 8 x 4 heads of 64, 1024 tokens: 88 + 111 us.
+// Bound: products and exponentials, which hardly overlap, and the clock.  4 x 16 heads of 128, 4096 tokens, causal, bf16, after a hundred passes: dQ 492 us (1120
+// TFLOP/s of its four products), dK / dV 515 us (1070); in the first ten 530 .. 557 and 570 .. 608 (the clock rises from 1.6 to 1.8 GHz of 2.4); matrix pipes busy
+// 61 / 57 % of the CUs' time, vector instructions 54 / 35 %, LDS 23 / 43 %, no bank conflicts.  fp32, 8 x 4 heads of 64, 1024 tokens: 75 + 94 us, first ten passes 88 + 111.
 // Roundings of bf16 tensors: dQ takes dS in TWO bf16 planes (a matrix instruction more on the same fragment): it is off by 1.65e-3 .. 1.85e-3 of its norm, of which its
 // own rounding is 1.65e-3 and delta from the rounded o up to 0.9e-3, in squares.  With one plane it was 2.5e-3, one and a half times what rounding the result
-// costs; the second plane is 7 % of a long training pass (4 x 16 heads of 128, 4096 tokens, causal: 1230 -> 1315 us; 7 padded samples 183 -> 195).  dK and dV round dS
+// costs; the second plane is 4 .. 7 % of a training pass (4 x 16 heads of 128, 4096 tokens, causal: 1256 -> 1305 us; 7 padded samples 184 -> 195).  dK and dV round dS
 // and P once (2.3e-3 .. 2.4e-3): a second plane finds no registers beside K, V and both accumulators.
 // Few tiles: the summed axis is split into ranges (grid `splits`), every range leaves an fp32 partial, mha_bwd_join_kernel adds them in order.
 // Row validity is decided where rows are staged: queries that do not exist or (causal) see no key come as zeros with lse = +inf, so P = 0 exactly and

@@ -6,11 +6,12 @@
 // Every lane holds 16 of a column's 32 scores: the row maximum is a register tree and one exchange with lane ^ 32, the sum stays per lane until the end.
 // The reference is the maximum (bf16: MH_LIFT above it) when it is set, and only moves when a tile's weights outgrow MH_GROW: then the accumulators are scaled.
 //
-// Bound: the matrix cores at the chip's power limit.  4 x 16 heads of 128, 4096 tokens, causal, bf16: 302 us (910 TFLOP/s; the library's 8192^3 product runs at
-// 1320), clock 1.63 GHz of 2.4, matrix pipes busy 54 % of the CUs' time, vector instructions 45 %, LDS 27 %, no bank conflicts.  4 x 8 heads of 64, 4096 tokens: 145 us
-// (950).  QB = 2 (64 rows a wave) halves the LDS reads a product and pays at D <= 64, where registers allow it (run back to back 162 us, with
-// QB = 1 173).
-// fp32, 8 x 4 heads of 64, 1024 tokens: 66 us (six products each: 780 TFLOP/s of bf16 work).
+// Bound: products and exponentials, which hardly overlap, and the clock.  4 x 16 heads of 128, 4096 tokens, causal, bf16: 272 us after a hundred passes (1010 TFLOP/s;
+// the library's 8192^3 product runs at 1320), 302 .. 313 us in the first ten (the clock rises from 1.6 to 1.8 GHz of 2.4); matrix pipes busy 54 % of the CUs' time,
+// vector instructions 45 %, LDS 27 %, no bank conflicts.  4 x 8 heads of 64, 4096 tokens: 144 us (957; first ten passes 159).  QB = 2 (64 rows a wave) halves the LDS
+// reads a product and pays at D <= 64, where registers allow it (both in their first passes: 162 us, with QB = 1 173).
+// fp32, 8 x 4 heads of 64, 1024 tokens: 57 us, first ten passes 67 (six products each: 904 TFLOP/s of bf16 work).  A head width that is no multiple of 8 loads single
+// elements and multiplies 128 channels: 4 x 8 heads, 1024 tokens, bf16 59 us at 20 channels, 16 at 24.
 //
 // Few rows (a token or a few per sample against a long cache): query heads that share a key head are rows of ONE tile (GP = G), and the keys are split into
 // ranges (grid `splits`), each leaving an unnormalised partial (O, m, l); the join kernels add them in a fixed order.

@@ -322,7 +322,7 @@ int pdae_attn_bwd(const float* qkv, const float* out, const float* lse, const fl
 int pdae_layernorm_fwd(const void* x, int64_t ldx, const float* gamma, const float* beta, int R, int C, float eps, void* y, int64_t ldy, float* mean, float* rstd,
                        int dtype, pdae_stream_t stream);
 /* dx = LayerNorm backward (+ add, the identity path around the norm); dgamma / dbeta (+)= sums over the rows, in a fixed order (acc_param selects "+=";
- * either may be NULL; with both NULL no workspace is needed).  dx may be add; no other output may overlap an input. */
+ * either may be NULL; with both NULL no workspace is needed).  dx may be add (with lddx = ldadd); no other output may overlap an input. */
 size_t pdae_layernorm_workspace_bytes(int R, int C);
 int pdae_layernorm_bwd(const void* x, int64_t ldx, const float* gamma, const float* mean, const float* rstd, const void* dy, int64_t lddy, const void* add,
                        int64_t ldadd, int R, int C, void* dx, int64_t lddx, float* dgamma, float* dbeta, int acc_param, void* ws, size_t ws_bytes, int dtype,

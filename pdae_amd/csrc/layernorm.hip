@@ -487,6 +487,7 @@ int k_layernorm_bwd(const void* x, long long ldx, const float* gamma, const floa
     PDAE_CHECK_ARG(!wg || (ws && ws_bytes >= k_layernorm_workspace_bytes(R, C)), "layernorm_bwd: weight gradients need %zu bytes of workspace (got %zu)",
                    k_layernorm_workspace_bytes(R, C), ws ? ws_bytes : (size_t)0);
     PDAE_CHECK_ARG(dx != x && dx != dy, "layernorm_bwd: dx in the place of x or dy (blocks of columns may still read them)");
+    PDAE_CHECK_ARG(dx != add || lddx == ldadd, "layernorm_bwd: dx in the place of add with another row stride");
     if (wg && ln_few(R, C)) {
       if (dtype == PDAE_DT_F32) ln_bwd_few<float>(x, ldx, gamma, mean, rstd, dy, lddy, add, ldadd, R, C, dx, lddx, dgamma, dbeta, acc_param, st);
       else ln_bwd_few<tk_bf16>(x, ldx, gamma, mean, rstd, dy, lddy, add, ldadd, R, C, dx, lddx, dgamma, dbeta, acc_param, st);

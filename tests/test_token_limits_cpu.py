@@ -53,6 +53,7 @@ def test_gradients_in_the_place_of_what_is_still_read_are_refused(H):
     refuses(H, bwd(P, Q, P), "in the place of")
     refuses(H, bwd(P, Q, Q), "in the place of")
     refuses(H, bwd(P, Q, Q, add=Q), "in the place of")
+    refuses(H, H.op_layernorm_bwd(P, P, P, P, Q, 4, 8, W, P, P, P, ws_bytes=1 << 20, add=W, lddx=9), "in the place of")      # dx may be add with one stride only
     a = H.Mha(2, 4, 4, 2, 2, 8)
     p = [P + 4096 * i for i in range(9)]
     for i in range(3):

@@ -32,6 +32,8 @@ def _on_device(name, first, *others):
 
 def _rows(x):
     """x as rows with contiguous channels: (tensor, rows, channels, row stride); a copy only when the strides do not allow rows."""
+    if x.dim() == 0:
+        raise H.PdaeError("layer_norm: a tensor of at least one dimension expected")
     C = x.shape[-1]
     if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= C:
         return x, x.shape[0], C, x.stride(0)

@@ -111,3 +111,10 @@ def test_layouts_the_kernels_take_are_not_copied():
     many = torch.empty_strided((1, 65, 2, 8), (0, 8, 1 << 27, 1), device="meta")       # 65 x 2 rows: heads are not packed
     assert tokens._heads(many, group=2) is many
     assert tokens._heads(meta(2, 4, 8, 2).transpose(2, 3)).is_contiguous()             # channels apart
+
+
+def test_layer_norm_of_a_scalar_is_refused(caught):
+    from pdae_amd import tokens
+    from pdae_amd.hip import PdaeError
+    with pytest.raises(PdaeError, match="dimension"):
+        tokens.layer_norm(torch.zeros(()))
